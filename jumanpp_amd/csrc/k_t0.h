@@ -301,7 +301,8 @@ __global__ void __launch_bounds__(64) k_t0(Batch B, const DevModel* __restrict__
 // instead of on the few lanes of pass A that missed.
 constexpr u32 kT0MissCap = 512;
 template <bool W24>
-__global__ void __launch_bounds__(64) k_t0_memo(Batch B, const DevModel* __restrict__ Mp, const T0Memo* __restrict__ memo, u32 nslots) {
+// (five wavefronts per SIMD as built with packed FP32 instructions; without them the allocator would stop at 99 registers, four)
+__global__ void __launch_bounds__(64) JPP_WAVES_PER_EU(5) k_t0_memo(Batch B, const DevModel* __restrict__ Mp, const T0Memo* __restrict__ memo, u32 nslots) {
   const DevModel& M = *Mp;
   const u32 s = blockIdx.x;
   if (B.sent_status[s] != ST_OK) return;
