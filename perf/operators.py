@@ -188,7 +188,7 @@ def _scan_train(gate, x, offsets, state, longest, dh, dlast):
     full, first, last = _ends(offsets)
     h, end = _scan(gate, x, offsets, state, longest)
     a, keep = torch.sigmoid(gate.float()), torch.sigmoid(-gate.float())
-    up = dh.float()
+    up = dh.float().clone()
     up[last] += dlast[full]
     after = torch.cat([a[1:], torch.zeros_like(a[:1])])
     after[last] = 0.0
