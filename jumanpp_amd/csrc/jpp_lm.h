@@ -1,0 +1,207 @@
+// Language-model operators: element types, packs of a row, the arithmetic they share.
+#ifndef JPP_LM_H
+#define JPP_LM_H
+
+#include <cmath>
+
+#include "jpp_rt.h"
+
+namespace jpp {
+
+// ---- elements ----------------------------------------------------------------
+// An element type is its storage and its way to and from 32 bits; nothing is computed in 16.
+struct LmF32 {
+  typedef float store;
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+};
+
+struct LmBf16 {
+  typedef u16 store;
+  static __device__ __forceinline__ float get(u16 v) {
+    const u32 w = (u32)v << 16;
+    float r;
+    __builtin_memcpy(&r, &w, 4);
+    return r;
+  }
+  static __device__ __forceinline__ u16 put(float v) {   // to nearest, ties to even
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_bit_cast(u16, (__bf16)v);
+#else
+    u32 w;
+    __builtin_memcpy(&w, &v, 4);
+    if (v != v) return (u16)((w >> 16) | 0x40u);
+    return (u16)((w + 0x7fffu + ((w >> 16) & 1u)) >> 16);
+#endif
+  }
+};
+
+struct LmF16 {
+  typedef u16 store;
+  static __device__ __forceinline__ float get(u16 v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return (float)__builtin_bit_cast(_Float16, v);
+#else
+    const u32 sign = (u32)(v & 0x8000u) << 16;
+    const int e = (v >> 10) & 31, m = v & 1023;
+    float r;
+    if (e == 31) r = m ? NAN : INFINITY;
+    else if (e == 0) r = std::ldexp((float)m, -24);
+    else r = std::ldexp((float)(m + 1024), e - 25);
+    return sign ? -r : r;
+#endif
+  }
+  static __device__ __forceinline__ u16 put(float v) {   // to nearest, ties to even
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_bit_cast(u16, (_Float16)v);
+#else
+    u32 w;
+    __builtin_memcpy(&w, &v, 4);
+    const u16 sign = (u16)((w >> 16) & 0x8000u);
+    const float a = std::fabs(v);
+    if (v != v) return (u16)(sign | 0x7e00u);
+    if (a == 0.f) return sign;
+    if (a >= 65520.f) return (u16)(sign | 0x7c00u);
+    int e = 0;
+    std::frexp(a, &e);                           // a < 2^e
+    const int ulp = e - 11 < -24 ? -24 : e - 11; // the last bit of a half of that size
+    const int m = (int)std::nearbyint(std::ldexp(a, -ulp));
+    const int be = ulp + 24;                     // 0 for subnormals and the lowest normal binade
+    return (u16)(sign | (u16)((be << 10) + m));  // (m >= 1024 carries into the exponent by itself)
+#endif
+  }
+};
+
+// N elements of a row, moved as one access of up to 16 bytes.  The pack has the alignment of its element: the global memory
+// path takes a wide access at any element's address, so rows of odd lengths and strides use the same loads (an access that
+// crosses a cache line costs a second look-up) and no kernel exists once per alignment.  A row whose length N does not
+// divide ends in a pack moved back to its last N elements: the lanes that share elements compute and store the same values.
+template <class T, int N>
+struct LmPack {
+  typename T::store v[N];
+};
+
+template <class T, int N>
+__device__ __forceinline__ LmPack<T, N> lm_load(const typename T::store* p) {
+  return *(const LmPack<T, N> JPP_GLOBAL*)p;
+}
+template <class T, int N>
+__device__ __forceinline__ void lm_store(typename T::store* p, const LmPack<T, N>& x) {
+  *(LmPack<T, N> JPP_GLOBAL*)p = x;
+}
+// first column of pack `i` of a row of dim >= N columns
+template <int N>
+__device__ __forceinline__ u32 lm_col(u32 i, u32 dim) {
+  const u32 c = i * N;
+  return N == 1 || c + N <= dim ? c : dim - N;
+}
+template <class T, int N>
+__device__ __forceinline__ LmPack<T, N> lm_pack(const float (&x)[N]) {
+  LmPack<T, N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = T::put(x[i]);
+  return r;
+}
+
+// ---- arithmetic ----------------------------------------------------------------
+__device__ __forceinline__ float lm_exp2(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_exp2f(x);   // (results below 2^-126 flush to zero: nothing here tells them from it)
+#else
+  return std::exp2(x);
+#endif
+}
+
+// 1 / d for 1 <= d <= 2: the reciprocal instruction and one Newton step (within half a unit and a bit)
+__device__ __forceinline__ float lm_rcp(float d) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const float r = __builtin_amdgcn_rcpf(d);
+  return __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
+#else
+  return 1.f / d;
+#endif
+}
+
+// exp(-y), y >= 0: 2^(-y log2 e).  The product's rounding and the digits of log2 e behind its 24th are put back to first
+// order (without either the relative error grows with y: 1e-6 at y = 20, and at y = 60).  NaN stays NaN, infinity gives 0.
+__device__ __forceinline__ float lm_exp_neg(float y) {
+  constexpr float kL = 1.44269504088896341f, kLlo = 1.92596303e-8f, kLn2 = 0.693147180559945309f;
+  const float t = -y * kL;
+  const float lo = __builtin_fmaf(-y, kLlo, __builtin_fmaf(-y, kL, -t));
+  const float e = lm_exp2(t);
+  return y > 104.f ? 0.f : __builtin_fmaf(e * lo, kLn2, e);
+}
+
+// a = sigmoid(z), b = 1 - a = sigmoid(-z), each to full relative precision: 1 - a would lose b's digits where the gate is
+// nearly open, and b is the weight of the input
+__device__ __forceinline__ void lm_gate(float z, float& a, float& b) {
+  const float e = lm_exp_neg(__builtin_fabsf(z));
+  const float r = lm_rcp(1.f + e), er = e * r;
+  const bool up = z >= 0.f;
+  a = up ? r : er;
+  b = up ? er : r;
+}
+
+// softplus(z) = max(z, 0) + ln(1 + exp(-|z|)), s = sigmoid(z); ln(1 + e) with the rounding of 1 + e put back
+__device__ __forceinline__ float lm_softplus(float z, float& s) {
+  const float e = lm_exp_neg(__builtin_fabsf(z));
+  const float u = 1.f + e;
+  const float r = lm_rcp(u);
+  s = z >= 0.f ? r : e * r;
+#if defined(__HIP_DEVICE_COMPILE__)
+  const float ln = __builtin_amdgcn_logf(u) * 0.693147180559945309f;   // (the instruction is a base-2 logarithm)
+#else
+  const float ln = std::log2(u) * 0.693147180559945309f;
+#endif
+  const float l = e < 0x1p-12f ? e - 0.5f * e * e : ln + (e - (u - 1.f)) * r;
+  return z != z ? z : (z > 0.f ? z : 0.f) + l;
+}
+
+template <int V>
+struct LmConst {
+  static constexpr int value = V;
+};
+
+// sum over aligned groups of N lanes (N = 4, 8, 16, 32 or 64), the same value in every lane of the group; the tree is
+// fixed, so the bits are
+template <int N>
+__device__ __forceinline__ float lm_group_sum(float v) {
+#if defined(JPP_EMU) || !defined(__HIP_DEVICE_COMPILE__)
+  for (int d = 1; d < N; d *= 2) v += wave_shfl_f32(v, lane_id() ^ d);
+  return v;
+#else
+  // inside rows of 16 lanes through DPP: quad permutes, half-row and row mirrors
+  auto dpp = [](float x, auto ctrl) {
+    int y;
+    __builtin_memcpy(&y, &x, 4);
+    y = __builtin_amdgcn_update_dpp(0, y, decltype(ctrl)::value, 0xf, 0xf, false);
+    __builtin_memcpy(&x, &y, 4);
+    return x;
+  };
+  if constexpr (N >= 2) v += dpp(v, LmConst<0xB1>());    // quad_perm 1,0,3,2
+  if constexpr (N >= 4) v += dpp(v, LmConst<0x4E>());    // quad_perm 2,3,0,1
+  if constexpr (N >= 8) v += dpp(v, LmConst<0x141>());   // row_half_mirror
+  if constexpr (N >= 16) v += dpp(v, LmConst<0x140>());  // row_mirror
+  if constexpr (N >= 32) v += wave_shfl_f32(v, lane_id() ^ 16);
+  if constexpr (N >= 64) v += wave_shfl_f32(v, lane_id() ^ 32);
+  return v;
+#endif
+}
+
+// ---- ids -----------------------------------------------------------------------
+struct LmIds {
+  const void* data;
+  u32 wide;   // int64 ids, not int32
+};
+// the id as a row of the table, or `vocab` where it names no word
+__device__ __forceinline__ u32 lm_row(const LmIds& ids, u64 i, u32 vocab) {
+  const i64 v = ids.wide ? as_global(static_cast<const i64*>(ids.data))[i] : (i64)as_global(static_cast<const i32*>(ids.data))[i];
+  return v >= 0 && v < (i64)vocab ? (u32)v : vocab;
+}
+
+constexpr u32 kLmThreads = 256;        // threads of a workgroup, where a kernel has no reason for another number
+constexpr u32 kLmMaxBlocks = 1u << 21; // largest grid (the sort of 2^31 entries has half of it); kernels that may need more loop
+
+}  // namespace jpp
+
+#endif  // JPP_LM_H

@@ -18,6 +18,7 @@
 #include <thread>
 #include <vector>
 
+#include "jpp_api.h"
 #include "jpp_rt.h"
 #include "jpp_types.h"
 #include "k_adjust.h"
@@ -931,6 +932,14 @@ ModelBufs::~ModelBufs() {
 }
 
 extern "C" const char* jppgpu_last_error(void) { return g_err.c_str(); }
+
+int jpp_api::fail(int code, const char* msg) noexcept {
+  try {
+    return ::fail(code, msg);
+  } catch (...) {   // (no memory for the message)
+    return code;
+  }
+}
 
 namespace {
 // Beams beyond kMaxBeam.  With the global beam on, a node's beam is filled from the boundary's global beam -- at most
