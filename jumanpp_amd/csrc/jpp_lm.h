@@ -12,97 +12,155 @@ namespace jpp {
 // An element type is its storage and its way to and from 32 bits; nothing is computed in 16.
 struct LmF32 {
   typedef float store;
-  static __device__ __forceinline__ float get(float v) { return v; }
-  static __device__ __forceinline__ float put(float v) { return v; }
+  static __device__ __forceinline__ float get(u32 bits) {
+    float r;
+    __builtin_memcpy(&r, &bits, 4);
+    return r;
+  }
+  static __device__ __forceinline__ u32 put(float v) {
+    u32 w;
+    __builtin_memcpy(&w, &v, 4);
+    return w;
+  }
 };
 
 struct LmBf16 {
   typedef u16 store;
-  static __device__ __forceinline__ float get(u16 v) {
-    const u32 w = (u32)v << 16;
-    float r;
-    __builtin_memcpy(&r, &w, 4);
-    return r;
-  }
-  static __device__ __forceinline__ u16 put(float v) {   // to nearest, ties to even
+  static __device__ __forceinline__ float get(u32 bits) { return LmF32::get(bits << 16); }
+  static __device__ __forceinline__ u32 put(float v) {   // to nearest, ties to even
 #if defined(__HIP_DEVICE_COMPILE__)
     return __builtin_bit_cast(u16, (__bf16)v);
 #else
-    u32 w;
-    __builtin_memcpy(&w, &v, 4);
-    if (v != v) return (u16)((w >> 16) | 0x40u);
-    return (u16)((w + 0x7fffu + ((w >> 16) & 1u)) >> 16);
+    const u32 w = LmF32::put(v);
+    if (v != v) return (w >> 16) | 0x40u;
+    return (w + 0x7fffu + ((w >> 16) & 1u)) >> 16;
 #endif
   }
 };
 
 struct LmF16 {
   typedef u16 store;
-  static __device__ __forceinline__ float get(u16 v) {
+  static __device__ __forceinline__ float get(u32 bits) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    return (float)__builtin_bit_cast(_Float16, v);
+    return (float)__builtin_bit_cast(_Float16, (u16)bits);
 #else
-    const u32 sign = (u32)(v & 0x8000u) << 16;
-    const int e = (v >> 10) & 31, m = v & 1023;
+    const int e = (bits >> 10) & 31, m = bits & 1023;
     float r;
     if (e == 31) r = m ? NAN : INFINITY;
     else if (e == 0) r = std::ldexp((float)m, -24);
     else r = std::ldexp((float)(m + 1024), e - 25);
-    return sign ? -r : r;
+    return (bits & 0x8000u) != 0 ? -r : r;
 #endif
   }
-  static __device__ __forceinline__ u16 put(float v) {   // to nearest, ties to even
+  static __device__ __forceinline__ u32 put(float v) {   // to nearest, ties to even
 #if defined(__HIP_DEVICE_COMPILE__)
     return __builtin_bit_cast(u16, (_Float16)v);
 #else
-    u32 w;
-    __builtin_memcpy(&w, &v, 4);
-    const u16 sign = (u16)((w >> 16) & 0x8000u);
+    const u32 sign = (LmF32::put(v) >> 16) & 0x8000u;
     const float a = std::fabs(v);
-    if (v != v) return (u16)(sign | 0x7e00u);
+    if (v != v) return sign | 0x7e00u;
     if (a == 0.f) return sign;
-    if (a >= 65520.f) return (u16)(sign | 0x7c00u);
+    if (a >= 65520.f) return sign | 0x7c00u;
     int e = 0;
     std::frexp(a, &e);                           // a < 2^e
     const int ulp = e - 11 < -24 ? -24 : e - 11; // the last bit of a half of that size
     const int m = (int)std::nearbyint(std::ldexp(a, -ulp));
     const int be = ulp + 24;                     // 0 for subnormals and the lowest normal binade
-    return (u16)(sign | (u16)((be << 10) + m));  // (m >= 1024 carries into the exponent by itself)
+    return sign | (u32)((be << 10) + m);         // (m >= 1024 carries into the exponent by itself)
 #endif
   }
 };
 
-// N elements of a row, moved as one access of up to 16 bytes.  The pack has the alignment of its element: the global memory
-// path takes a wide access at any element's address, so rows of odd lengths and strides use the same loads (an access that
-// crosses a cache line costs a second look-up) and no kernel exists once per alignment.  A row whose length N does not
-// divide ends in a pack moved back to its last N elements: the lanes that share elements compute and store the same values.
+// N elements of a row, moved as one access of up to 16 bytes and held as the words that came.  (Held as an array of 16-bit
+// elements, a pack that is loaded under a condition is taken apart inside the branch, behind a wait of its own.)  The access
+// asks for no more alignment than an element has: the global memory path takes a wide one at any element's address, so rows
+// of odd lengths and strides use the same loads (one that crosses a cache line costs a second look-up) and no kernel exists
+// once per alignment.
 template <class T, int N>
 struct LmPack {
-  typename T::store v[N];
+  static constexpr int kBytes = N * (int)sizeof(typename T::store), kWords = (kBytes + 3) / 4;
+  u32 w[kWords];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(typename T::store) == 4) return T::get(w[i]);
+    else return T::get((i & 1) != 0 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+  }
+  __device__ __forceinline__ void set(const float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(typename T::store) == 4) w[i] = T::put(x[i]);
+      else w[i] = T::put(x[2 * i]) | (2 * i + 1 < N ? T::put(x[2 * i + 1 < N ? 2 * i + 1 : 0]) << 16 : 0u);
+    }
+  }
 };
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// the register image of a pack, with the alignment of an element
+template <int BYTES, int ALIGN>
+struct LmRaw {
+  typedef u32 type __attribute__((ext_vector_type(BYTES / 4), aligned(ALIGN)));
+};
+template <>
+struct LmRaw<4, 4> {
+  typedef u32 type;
+};
+template <>
+struct LmRaw<4, 2> {
+  typedef u32 type __attribute__((aligned(2)));
+};
+template <>
+struct LmRaw<2, 2> {
+  typedef u16 type;
+};
+#endif
 
 template <class T, int N>
 __device__ __forceinline__ LmPack<T, N> lm_load(const typename T::store* p) {
-  return *(const LmPack<T, N> JPP_GLOBAL*)p;
+  LmPack<T, N> x;
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef typename LmRaw<LmPack<T, N>::kBytes, sizeof(typename T::store)>::type Raw;
+  const Raw r = *(const Raw JPP_GLOBAL*)p;
+  if constexpr (LmPack<T, N>::kBytes == 2) x.w[0] = r;
+  else __builtin_memcpy(&x, &r, sizeof(x));
+#else
+  x.w[LmPack<T, N>::kWords - 1] = 0;
+  __builtin_memcpy(&x, p, LmPack<T, N>::kBytes);
+#endif
+  return x;
+}
+// STREAM: with the non-temporal hint, for results too large to be found in a cache by whoever reads them, so that they do not
+// push out what this kernel itself reads again.  (A template argument: two stores under a condition that differ in the hint
+// alone are merged into one without it.)
+template <class T, int N, bool STREAM = false>
+__device__ __forceinline__ void lm_store(typename T::store* p, const LmPack<T, N>& x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef typename LmRaw<LmPack<T, N>::kBytes, sizeof(typename T::store)>::type Raw;
+  Raw r;
+  if constexpr (LmPack<T, N>::kBytes == 2) r = (Raw)x.w[0];
+  else __builtin_memcpy(&r, &x, sizeof(x));
+  if constexpr (STREAM) __builtin_nontemporal_store(r, (Raw JPP_GLOBAL*)p);
+  else *(Raw JPP_GLOBAL*)p = r;
+#else
+  __builtin_memcpy(p, &x, LmPack<T, N>::kBytes);
+#endif
 }
 template <class T, int N>
-__device__ __forceinline__ void lm_store(typename T::store* p, const LmPack<T, N>& x) {
-  *(LmPack<T, N> JPP_GLOBAL*)p = x;
+__device__ __forceinline__ LmPack<T, N> lm_pack(const float (&x)[N]) {
+  LmPack<T, N> r;
+  r.set(x);
+  return r;
 }
+// A row whose length N does not divide ends in a pack moved back to its last N elements: the lanes that share elements
+// compute and store the same values.
 // first column of pack `i` of a row of dim >= N columns
 template <int N>
 __device__ __forceinline__ u32 lm_col(u32 i, u32 dim) {
   const u32 c = i * N;
   return N == 1 || c + N <= dim ? c : dim - N;
 }
-template <class T, int N>
-__device__ __forceinline__ LmPack<T, N> lm_pack(const float (&x)[N]) {
-  LmPack<T, N> r;
-#pragma unroll
-  for (int i = 0; i < N; ++i) r.v[i] = T::put(x[i]);
-  return r;
-}
-
 // ---- arithmetic ----------------------------------------------------------------
 __device__ __forceinline__ float lm_exp2(float x) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -200,6 +258,7 @@ __device__ __forceinline__ u32 lm_row(const LmIds& ids, u64 i, u32 vocab) {
 }
 
 constexpr u32 kLmThreads = 256;        // threads of a workgroup, where a kernel has no reason for another number
+constexpr u64 kLmChipBlocks = 256 * 8; // workgroups of kLmThreads threads that the 256 compute units hold at most
 constexpr u32 kLmMaxBlocks = 1u << 21; // largest grid (the sort of 2^31 entries has half of it); kernels that may need more loop
 
 }  // namespace jpp

@@ -84,6 +84,10 @@ struct Launcher {
   }
 };
 
+// Results of more bytes than this leave with the non-temporal hint.
+constexpr u64 kStreamBytes = u64{64} << 20;
+bool streamed(u64 bytes) { return bytes > kStreamBytes; }
+
 u64 div_up(u64 a, u64 b) { return (a + b - 1) / b; }
 
 // ---- checks --------------------------------------------------------------------------
@@ -280,18 +284,22 @@ void clear_matrix(Launcher& go, const jppgpu_lm_matrix* m, u64 rows, u64 cols) {
   go(k_lm_zero, zero_blocks(z), kLmThreads, z);
 }
 
+template <class Tin, class Tout, int V, int PER, bool STREAM>
+void launch_embed_packs(Launcher& go, const jppgpu_lm_matrix* table, u32 vocab, u32 dim, LmIds ids, u64 n, float scale, const jppgpu_lm_matrix* out) {
+  const u32 packs = (u32)div_up(dim, V), per = PER * kLmThreads;
+  const u32 rows = packs >= per ? 1 : per / packs;
+  go(k_lm_embed<Tin, Tout, V, PER, STREAM>, div_up(n, rows), kLmThreads, static_cast<const typename Tin::store*>(table->data), table->stride,
+     vocab, dim, ids, n, scale, static_cast<typename Tout::store*>(out->data), out->stride, rows);
+}
+
 template <class Tin, class Tout>
 void launch_embed(Launcher& go, const jppgpu_lm_matrix* table, u32 vocab, u32 dim, LmIds ids, u64 n, float scale, const jppgpu_lm_matrix* out) {
-  constexpr u32 V = 16 / sizeof(typename Tin::store);
-  const u32 packs = dim >= V ? (u32)div_up(dim, V) : dim;
-  // a pack a thread while that fills the chip's wavefront slots at most once, four from there on
-  const u64 total = n * packs;
-  const u32 per = total < (u64)256 * 2048 ? kLmThreads : 4 * kLmThreads;
-  const u32 rows = packs >= per ? 1 : per / packs;
-  auto t = static_cast<const typename Tin::store*>(table->data);
-  auto o = static_cast<typename Tout::store*>(out->data);
-  if (dim >= V) go(k_lm_embed<Tin, Tout, (int)V>, div_up(n, rows), kLmThreads, t, table->stride, vocab, dim, ids, n, scale, o, out->stride, rows);
-  else go(k_lm_embed<Tin, Tout, 1>, div_up(n, rows), kLmThreads, t, table->stride, vocab, dim, ids, n, scale, o, out->stride, rows);
+  constexpr int V = 16 / sizeof(typename Tout::store);   // a 16-byte store a lane
+  // four packs a thread once that still fills the chip's wavefront slots
+  if (dim < (u32)V) launch_embed_packs<Tin, Tout, 1, 1, false>(go, table, vocab, dim, ids, n, scale, out);
+  else if (n * div_up(dim, V) < (u64)4 * 256 * 2048) launch_embed_packs<Tin, Tout, V, 1, false>(go, table, vocab, dim, ids, n, scale, out);
+  else if (!streamed(n * dim * sizeof(typename Tout::store))) launch_embed_packs<Tin, Tout, V, 4, false>(go, table, vocab, dim, ids, n, scale, out);
+  else launch_embed_packs<Tin, Tout, V, 4, true>(go, table, vocab, dim, ids, n, scale, out);
 }
 
 // ---- the recurrence --------------------------------------------------------------------
@@ -314,33 +322,45 @@ u32 scan_chunk(u64 rows, u64 n, u64 dim, u64 maxLen) {
   return (u32)(chunk < 32 ? 32 : chunk);
 }
 
-template <class T, int V>
+template <class T, int V, bool STREAM>
 void launch_scan(Launcher& go, const LmScan<T>& q) {
   const u64 waves = kLmThreads / 64;
   if (q.chunk == 0) {
     const u64 blocks = div_up((u64)q.n * q.colBlocks, waves);
-    if (q.saved != nullptr) go(k_lm_scan_seq<T, V, true>, blocks, kLmThreads, q);
-    else go(k_lm_scan_seq<T, V, false>, blocks, kLmThreads, q);
+    if (q.saved != nullptr) go(k_lm_scan_seq<T, V, true, STREAM>, blocks, kLmThreads, q);
+    else go(k_lm_scan_seq<T, V, false, STREAM>, blocks, kLmThreads, q);
     return;
   }
   const u64 blocks = div_up((u64)q.chunks * q.colBlocks, waves);
   go(k_lm_scan_agg<T, V>, blocks, kLmThreads, q);
   go(k_lm_scan_carry<false>, div_up(q.dim, 64), 64u * kLmCarryWaves, q.aggA, q.aggB, q.chunks, q.dim);
-  if (q.saved != nullptr) go(k_lm_scan_chunk<T, V, true>, blocks, kLmThreads, q);
-  else go(k_lm_scan_chunk<T, V, false>, blocks, kLmThreads, q);
+  if (q.saved != nullptr) go(k_lm_scan_chunk<T, V, true, STREAM>, blocks, kLmThreads, q);
+  else go(k_lm_scan_chunk<T, V, false, STREAM>, blocks, kLmThreads, q);
 }
 
-template <class T, int V>
+template <class T, int V, bool STREAM>
 void launch_scan_grad(Launcher& go, const LmScan<T>& q) {
   const u64 waves = kLmThreads / 64;
   if (q.chunk == 0) {
-    go(k_lm_scan_grad_seq<T, V>, div_up((u64)q.n * q.colBlocks, waves), kLmThreads, q);
+    go(k_lm_scan_grad_seq<T, V, STREAM>, div_up((u64)q.n * q.colBlocks, waves), kLmThreads, q);
     return;
   }
   const u64 blocks = div_up((u64)q.chunks * q.colBlocks, waves);
   go(k_lm_scan_grad_agg<T, V>, blocks, kLmThreads, q);
   go(k_lm_scan_carry<true>, div_up(q.dim, 64), 64u * kLmCarryWaves, q.aggA, q.aggB, q.chunks, q.dim);
-  go(k_lm_scan_grad_chunk<T, V>, blocks, kLmThreads, q);
+  go(k_lm_scan_grad_chunk<T, V, STREAM>, blocks, kLmThreads, q);
+}
+
+template <class T, int V>
+void launch_scan_any(Launcher& go, const LmScan<T>& q, bool grad) {
+  const bool stream = streamed((u64)q.rows * q.dim * sizeof(typename T::store));
+  if (!grad) {
+    if (stream) launch_scan<T, V, true>(go, q);
+    else launch_scan<T, V, false>(go, q);
+  } else if constexpr (V * sizeof(typename T::store) <= 8) {
+    if (stream) launch_scan_grad<T, V, true>(go, q);
+    else launch_scan_grad<T, V, false>(go, q);
+  }
 }
 
 struct ScanArgs {
@@ -400,15 +420,9 @@ void run_scan(Launcher& go, const ScanArgs& s, bool grad) {
     q.aggA = c.take<float>((u64)q.chunks * q.dim);
     q.aggB = c.take<float>((u64)q.chunks * q.dim);
   }
-  if (!grad) {
-    if (v == 1) launch_scan<T, 1>(go, q);
-    else if (v == 2) launch_scan<T, 2>(go, q);
-    else launch_scan<T, 4>(go, q);
-  } else {
-    if (v == 1) launch_scan_grad<T, 1>(go, q);
-    else if (v == 2) launch_scan_grad<T, 2>(go, q);
-    else if constexpr (sizeof(S) == 2) launch_scan_grad<T, 4>(go, q);
-  }
+  if (v == 1) launch_scan_any<T, 1>(go, q, grad);
+  else if (v == 2) launch_scan_any<T, 2>(go, q, grad);
+  else launch_scan_any<T, 4>(go, q, grad);
 }
 
 int check_scan(const ScanArgs& s) {
@@ -436,26 +450,37 @@ uint64_t scan_workspace(int64_t rows, int64_t n, int64_t dim, int64_t max_len) {
 }
 
 // ---- noise-contrastive score and loss ------------------------------------------------------
-template <class T, int G, int NV, bool BLOCKS>
+template <class T, int G, int NV, LmRowKind KIND>
 void launch_nce(Launcher& go, const LmNce& q, const void* h, const void* table, LmIds ids, void* dh, bool loss) {
   constexpr int V = 16 / (int)sizeof(typename T::store);
   auto hp = static_cast<const typename T::store*>(h);
   auto tp = static_cast<const typename T::store*>(table);
   auto dp = static_cast<typename T::store*>(dh);
-  if (!loss) go(k_lm_nce_score<T, V, G, NV, BLOCKS>, div_up(q.n * q.cands, kLmThreads / G), kLmThreads, q, hp, tp, ids);
-  else if (dp != nullptr) go(k_lm_nce_loss<T, V, G, NV, BLOCKS, true>, div_up(q.n, kLmThreads / 64), kLmThreads, q, hp, tp, ids, dp);
-  else go(k_lm_nce_loss<T, V, G, NV, BLOCKS, false>, div_up(q.n, kLmThreads / 64), kLmThreads, q, hp, tp, ids, dp);
+  if (!loss) {
+    go(k_lm_nce_score<T, V, G, NV, KIND>, div_up(q.n * div_up(q.cands, kLmScoreCands), kLmThreads / G), kLmThreads, q, hp, tp, ids);
+    return;
+  }
+  // no more workgroups than fit the chip at once: a wavefront that goes from token to token has the next one's data ahead
+  const u64 blocks = div_up(q.n, kLmThreads / 64), most = blocks < kLmChipBlocks ? blocks : kLmChipBlocks;
+  if (dp != nullptr) go(k_lm_nce_loss<T, V, G, NV, KIND, true>, most, kLmThreads, q, hp, tp, ids, dp);
+  else go(k_lm_nce_loss<T, V, G, NV, KIND, false>, most, kLmThreads, q, hp, tp, ids, dp);
+}
+
+template <class T, int G, int NV>
+void launch_nce_row(Launcher& go, const LmNce& q, const void* h, const void* table, LmIds ids, void* dh, bool loss) {
+  if (q.dim == G * NV * (16 / sizeof(typename T::store))) launch_nce<T, G, NV, kLmFull>(go, q, h, table, ids, dh, loss);
+  else launch_nce<T, G, NV, kLmPart>(go, q, h, table, ids, dh, loss);
 }
 
 template <class T>
 void run_nce(Launcher& go, const LmNce& q, const void* h, const void* table, LmIds ids, void* dh, bool loss) {
   const u32 packs = q.dim / (16 / (u32)sizeof(typename T::store));
-  if (packs <= 16) launch_nce<T, 16, 1, false>(go, q, h, table, ids, dh, loss);
-  else if (packs <= 32) launch_nce<T, 16, 2, false>(go, q, h, table, ids, dh, loss);
-  else if (packs <= 64) launch_nce<T, 16, 4, false>(go, q, h, table, ids, dh, loss);
-  else if (packs <= 128) launch_nce<T, 64, 2, false>(go, q, h, table, ids, dh, loss);
-  else if (packs <= 256) launch_nce<T, 64, 4, false>(go, q, h, table, ids, dh, loss);
-  else launch_nce<T, 64, 4, true>(go, q, h, table, ids, dh, loss);
+  if (packs <= 16) launch_nce_row<T, 16, 1>(go, q, h, table, ids, dh, loss);
+  else if (packs <= 32) launch_nce_row<T, 16, 2>(go, q, h, table, ids, dh, loss);
+  else if (packs <= 64) launch_nce_row<T, 16, 4>(go, q, h, table, ids, dh, loss);
+  else if (packs <= 128) launch_nce_row<T, 64, 2>(go, q, h, table, ids, dh, loss);
+  else if (packs <= 256) launch_nce_row<T, 64, 4>(go, q, h, table, ids, dh, loss);
+  else launch_nce<T, 64, 4, kLmBlocks>(go, q, h, table, ids, dh, loss);
 }
 
 void dispatch_nce(Launcher& go, const LmNce& q, const jppgpu_lm_matrix* h, const jppgpu_lm_matrix* table, LmIds ids, void* dh, bool loss) {

@@ -20,30 +20,40 @@ namespace jpp {
 
 // ---- lookup --------------------------------------------------------------------
 // y_t = scale * W[id_t].  A thread moves packs of V elements, a workgroup `rowsPerBlock` rows; nothing but the loads and
-// stores counts.
-template <class Tin, class Tout, int V>
+// stores counts.  The ids of PER packs are loaded together, then their rows: one wait each, not one a pack.
+template <class Tin, class Tout, int V, int PER, bool STREAM>
 __global__ void __launch_bounds__(kLmThreads)
-    k_lm_embed(const typename Tin::store* __restrict__ table, i64 tableStride, u32 vocab, u32 dim, LmIds ids, u64 n,
-               float scale, typename Tout::store* __restrict__ out, i64 outStride, u32 rowsPerBlock) {
+    k_lm_embed(const typename Tin::store* __restrict__ table, i64 tableStride, u32 vocab, u32 dim, LmIds ids, u64 n, float scale,
+               typename Tout::store* __restrict__ out, i64 outStride, u32 rowsPerBlock) {
   const u32 packs = (dim + V - 1) / V;
   const u64 groups = (n + rowsPerBlock - 1) / rowsPerBlock;
   for (u64 g = blockIdx.x; g < groups; g += gridDim.x) {
     const u64 t0 = g * rowsPerBlock;
     const u32 rows = n - t0 < rowsPerBlock ? (u32)(n - t0) : rowsPerBlock;
     const u32 total = rows * packs;
-#pragma unroll 4
-    for (u32 i = threadIdx.x; i < total; i += kLmThreads) {
-      const u32 r = i / packs, c = lm_col<V>(i - r * packs, dim);
-      const u32 row = lm_row(ids, t0 + r, vocab);
-      float y[V];
+    for (u32 i0 = threadIdx.x; i0 < total; i0 += kLmThreads * PER) {
+      u32 r[PER], c[PER], row[PER];
+      LmPack<Tin, V> x[PER];
 #pragma unroll
-      for (int e = 0; e < V; ++e) y[e] = 0.f;
-      if (row < vocab) {
-        const LmPack<Tin, V> x = lm_load<Tin, V>(table + (i64)row * tableStride + c);
-#pragma unroll
-        for (int e = 0; e < V; ++e) y[e] = Tin::get(x.v[e]) * scale;
+      for (int k = 0; k < PER; ++k) {
+        const u32 i = i0 + (u32)k * kLmThreads < total ? i0 + (u32)k * kLmThreads : i0;
+        r[k] = i / packs;
+        c[k] = lm_col<V>(i - r[k] * packs, dim);
+        row[k] = lm_row(ids, t0 + r[k], vocab);
       }
-      lm_store<Tout, V>(out + (i64)(t0 + r) * outStride + c, lm_pack<Tout, V>(y));
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        x[k].zero();
+        // (an id that names no word reads row 0, if there is one, for nothing)
+        if (vocab != 0) x[k] = lm_load<Tin, V>(table + (i64)(row[k] < vocab ? row[k] : 0u) * tableStride + c[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        float y[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = row[k] < vocab ? x[k].get(e) * scale : 0.f;
+        if (i0 + (u32)k * kLmThreads < total) lm_store<Tout, V, STREAM>(out + (i64)(t0 + r[k]) * outStride + c[k], lm_pack<Tout, V>(y));
+      }
     }
   }
 }
@@ -61,7 +71,8 @@ __device__ __forceinline__ void lm_zero_rows(const LmZero& z, u64 first, u64 ste
     float* row = z.data + (i64)r * z.stride;
     const u32 cols = r + 1 == z.rows ? z.lastCols : z.cols;
     const u32 packs = cols / 4;
-    const LmPack<LmF32, 4> zero = {{0.f, 0.f, 0.f, 0.f}};
+    LmPack<LmF32, 4> zero;
+    zero.zero();
     for (u32 c = threadIdx.x; c < packs; c += blockDim.x) lm_store<LmF32, 4>(row + 4 * (u64)c, zero);
     for (u32 c = packs * 4 + threadIdx.x; c < cols; c += blockDim.x) row[c] = 0.f;
   }
@@ -336,11 +347,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_seg_sum(LmSeg q, const typena
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.f;
     auto put = [&](float* row) {
-      if (!on) return;
-      LmPack<LmF32, V> o;
-#pragma unroll
-      for (int e = 0; e < V; ++e) o.v[e] = acc[e];
-      lm_store<LmF32, V>(row + col, o);
+      if (on) lm_store<LmF32, V>(row + col, lm_pack<LmF32, V>(acc));
     };
     for (u32 i0 = 0; i0 < cnt && cur < q.vocab; i0 += 8) {
       LmPack<T, V> x[8];
@@ -365,7 +372,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_seg_sum(LmSeg q, const typena
           }
           if (key < q.vocab) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] = __builtin_fmaf(wi, T::get(x[i].v[e]), acc[e]);
+            for (int e = 0; e < V; ++e) acc[e] = __builtin_fmaf(wi, x[i].get(e), acc[e]);
           }
         }
       }

@@ -30,30 +30,42 @@ struct LmNce {
 
 // A lane's part of a row: packs l, l + G, ... of V elements (from pack `p0` on, `packs` in the row) and, where V does not
 // divide the row, one of its last elements.  Parts that do not exist are zero, so a product over the group counts every
-// element once.
+// element once; they are loaded from the row's start and cleared (no branch, so that a wait covers many rows).  FULL: every
+// part exists.
 struct LmRowShape {
   u32 packs, rest;   // full packs, elements behind them
 };
-template <class T, int V, int G, int NV>
+template <class T, int V, int G, int NV, bool FULL>
 struct LmRowPart {
   LmPack<T, V> p[NV];
-  typename T::store tail;
+  LmPack<T, 1> tail;
   __device__ __forceinline__ void load(const typename T::store* row, u32 p0, u32 gl, const LmRowShape& s) {
+    if constexpr (FULL) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const u32 at = p0 + gl + (u32)(G * i);
-      if (at < s.packs) {
-        p[i] = lm_load<T, V>(row + at * V);
-      } else {
+      for (int i = 0; i < NV; ++i) p[i] = lm_load<T, V>(row + (gl + (u32)(G * i)) * V);
+      tail.zero();
+    } else {
+      // (where V > dim there is no full pack: the tail has it all)
 #pragma unroll
-        for (int e = 0; e < V; ++e) p[i].v[e] = 0;
+      for (int i = 0; i < NV; ++i) {
+        p[i].zero();
+        if (s.packs != 0) p[i] = lm_load<T, V>(row + (p0 + gl + (u32)(G * i) < s.packs ? p0 + gl + (u32)(G * i) : 0u) * V);
       }
+      tail.zero();
+      if (s.rest != 0) tail = lm_load<T, 1>(row + s.packs * V + (gl < s.rest ? gl : 0u));
     }
-    tail = 0;
-    if (s.rest != 0 && p0 == 0 && gl < s.rest) tail = as_global(row)[s.packs * V + gl];
+  }
+  __device__ __forceinline__ void mask(u32 p0, u32 gl, const LmRowShape& s) {
+    if constexpr (!FULL) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < LmPack<T, V>::kWords; ++k) p[i].w[k] = p0 + gl + (u32)(G * i) < s.packs ? p[i].w[k] : 0u;
+      tail.w[0] = p0 == 0 && gl < s.rest ? tail.w[0] : 0u;
+    }
   }
 };
-template <int V, int NV>
+template <int V, int NV, bool FULL>
 struct LmRowSum {    // the same part in 32 bits
   float p[NV][V];
   float tail;
@@ -65,20 +77,21 @@ struct LmRowSum {    // the same part in 32 bits
     tail = 0.f;
   }
   template <class T, int G>
-  __device__ __forceinline__ void add(float w, const LmRowPart<T, V, G, NV>& x) {
+  __device__ __forceinline__ void add(float w, const LmRowPart<T, V, G, NV, FULL>& x) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < V; ++e) p[i][e] = __builtin_fmaf(w, T::get(x.p[i].v[e]), p[i][e]);
-    tail = __builtin_fmaf(w, T::get(x.tail), tail);
+      for (int e = 0; e < V; ++e) p[i][e] = __builtin_fmaf(w, x.p[i].get(e), p[i][e]);
+    if constexpr (!FULL) tail = __builtin_fmaf(w, x.tail.get(0), tail);
   }
   template <class T, int G>
-  __device__ __forceinline__ float dot(const LmRowPart<T, V, G, NV>& x) const {
-    float d = tail * T::get(x.tail);
+  __device__ __forceinline__ float dot(const LmRowPart<T, V, G, NV, FULL>& x) const {
+    float d = 0.f;
+    if constexpr (!FULL) d = tail * x.tail.get(0);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < V; ++e) d = __builtin_fmaf(p[i][e], T::get(x.p[i].v[e]), d);
+      for (int e = 0; e < V; ++e) d = __builtin_fmaf(p[i][e], x.p[i].get(e), d);
     return d;
   }
   template <class T, int G>
@@ -86,116 +99,206 @@ struct LmRowSum {    // the same part in 32 bits
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const u32 at = p0 + gl + (u32)(G * i);
-      if (at < s.packs) lm_store<T, V>(row + at * V, lm_pack<T, V>(p[i]));
+      if (FULL || at < s.packs) lm_store<T, V>(row + at * V, lm_pack<T, V>(p[i]));
     }
-    if (s.rest != 0 && p0 == 0 && gl < s.rest) ((typename T::store JPP_GLOBAL*)row)[s.packs * V + gl] = T::put(tail);
+    if (!FULL && s.rest != 0 && p0 == 0 && gl < s.rest) {
+      const float x[1] = {tail};
+      lm_store<T, 1>(row + s.packs * V + gl, lm_pack<T, 1>(x));
+    }
   }
 };
 
-// NV packs of V elements a lane cover G NV packs; BLOCKS: the row has more and is walked in such blocks (the loss then reads
-// the rows of W twice)
-template <class T, int V, int G, int NV, bool BLOCKS>
-__global__ void __launch_bounds__(kLmThreads)
-    k_lm_nce_score(LmNce q, const typename T::store* __restrict__ h, const typename T::store* __restrict__ table, LmIds ids) {
-  const u32 gl = threadIdx.x & (G - 1);
-  const LmRowShape shape = {q.dim / V, q.dim % V};
-  const u64 pairs = q.n * q.cands;
-  const u64 step = (u64)gridDim.x * (kLmThreads / G);
-  // (whole wavefronts stay in the loop: the group sums are wavefront operations)
-  for (u64 j0 = (u64)blockIdx.x * (kLmThreads / G); j0 < pairs; j0 += step) {
-    const u64 j = j0 + threadIdx.x / G;
-    const u32 row = j < pairs ? lm_row(ids, j, q.vocab) : q.vocab;
-    const u64 t = j < pairs ? (pairs <= 0xffffffffu ? (u64)((u32)j / q.cands) : j / q.cands) : 0u;
-    float dot = 0.f;
-    if (row < q.vocab) {
-      for (u32 p0 = 0; p0 < (BLOCKS ? shape.packs : 1u); p0 += G * NV) {
-        LmRowPart<T, V, G, NV> a, b;
-        a.load(h + (i64)t * q.hStride, p0, gl, shape);
-        b.load(table + (i64)row * q.tableStride, p0, gl, shape);
-        LmRowSum<V, NV> x;
-        x.zero();
-        x.template add<T, G>(1.f, a);
-        dot += x.template dot<T, G>(b);
-      }
-    }
-    dot = lm_group_sum<G>(dot);
-    if (gl == 0 && j < pairs) q.out[j] = row < q.vocab ? dot - q.constant : -__builtin_inff();
+// the product of two rows, block of columns by block
+template <class T, int V, int G, int NV>
+__device__ __forceinline__ float lm_dot_blocks(const typename T::store* x, const typename T::store* y, u32 gl, const LmRowShape& s) {
+  float d = 0.f;
+  for (u32 p0 = 0; p0 < s.packs; p0 += G * NV) {
+    LmRowPart<T, V, G, NV, false> a, b;
+    a.load(x, p0, gl, s);
+    b.load(y, p0, gl, s);
+    a.mask(p0, gl, s);
+    b.mask(p0, gl, s);
+    LmRowSum<V, NV, false> f;
+    f.zero();
+    f.template add<T, G>(1.f, a);
+    d += f.template dot<T, G>(b);
   }
+  return d;
 }
 
-template <class T, int V, int G, int NV, bool BLOCKS, bool DH>
+// NV packs of V elements a lane cover G NV packs: the whole row exactly (kLmFull), the whole row (kLmPart), or a block of it,
+// the row being longer (kLmBlocks: the loss then reads the rows of W twice).
+enum LmRowKind { kLmFull, kLmPart, kLmBlocks };
+// Rows in flight a group: about 32 registers of them.
+template <class T, int V, int NV>
+constexpr int lm_rows_in_flight() {
+  return NV * V * (int)sizeof(typename T::store) >= 64 ? 2 : NV * V * (int)sizeof(typename T::store) >= 32 ? 4 : 8;
+}
+
+// A group takes up to kLmScoreCands candidates of a token: h comes in once for them, their ids with one load (a lane each),
+// their rows several at a time.  The vector unit decides: where a row starts is worked out once, by the lane that loaded the
+// id (a 64-bit product is a dozen full-rate operations), and handed to the group.
+constexpr u32 kLmScoreCands = 16;
+template <class T, int V, int G, int NV, LmRowKind KIND>
 __global__ void __launch_bounds__(kLmThreads)
-    k_lm_nce_loss(LmNce q, const typename T::store* __restrict__ h, const typename T::store* __restrict__ table, LmIds ids,
-                  typename T::store* __restrict__ dh) {
-  constexpr u32 kGroups = 64 / G;
-  constexpr int U = NV * V >= 32 ? 1 : NV * V >= 16 ? 2 : 4;   // candidates of a group in flight
+    k_lm_nce_score(LmNce q, const typename T::store* __restrict__ h, const typename T::store* __restrict__ table, LmIds ids) {
+  constexpr bool BLOCKS = KIND == kLmBlocks, FULL = KIND == kLmFull;
+  constexpr int U = BLOCKS ? 1 : lm_rows_in_flight<T, V, NV>();
   const int lane = (int)(threadIdx.x & 63);
-  const u32 gl = threadIdx.x & (G - 1), grp = (u32)lane / G;
+  const u32 gl = threadIdx.x & (G - 1);
   const LmRowShape shape = {q.dim / V, q.dim % V};
-  for (u64 t = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6); t < q.n; t += (u64)gridDim.x * (kLmThreads / 64)) {
-    const u32 target = uni(lm_row(ids, t * q.cands, q.vocab));
-    const bool live = target < q.vocab;
-    const float w = q.weight != nullptr ? q.weight[t] : 1.f;
-    LmRowSum<V, NV> hr, acc;
-    hr.zero();
-    acc.zero();
-    float loss = 0.f;
-    if (live && !BLOCKS) {
-      LmRowPart<T, V, G, NV> a;
-      a.load(h + (i64)t * q.hStride, 0, gl, shape);
-      hr.template add<T, G>(1.f, a);
-    }
-    for (u32 kb = 0; live && kb < q.cands; kb += 64) {
-      // the rows of 64 candidates, a lane each, ahead of the gathers that need them
-      const u32 kn = q.cands - kb < 64 ? q.cands - kb : 64u;
-      u32 rowL = q.vocab;
-      if ((u32)lane < kn) rowL = lm_row(ids, t * q.cands + kb + (u32)lane, q.vocab);
-      const float biasL = rowL < q.vocab ? q.constant + q.logNoise[rowL] : 0.f;
-      float gL = 0.f;
-      for (u32 k0 = 0; k0 < kn; k0 += kGroups * U) {
-        LmRowPart<T, V, G, NV> b[U];
-        u32 row[U];
+  const u32 parts = (q.cands + kLmScoreCands - 1) / kLmScoreCands;
+  const u64 tasks = q.n * parts;
+  const u64 step = (u64)gridDim.x * (kLmThreads / G);
+  // (whole wavefronts stay in the loop: the group sums are wavefront operations)
+  for (u64 task0 = (u64)blockIdx.x * (kLmThreads / G); task0 < tasks; task0 += step) {
+    const u64 task = task0 + threadIdx.x / G;
+    const bool some = task < tasks;
+    const u64 t = some ? (parts == 1 ? task : task / parts) : 0u;
+    const u32 k0 = some ? (u32)(task - t * parts) * kLmScoreCands : 0u;
+    const u32 cnt = some ? (q.cands - k0 < kLmScoreCands ? q.cands - k0 : kLmScoreCands) : 0u;
+    const u32 rowL = gl < cnt ? lm_row(ids, t * q.cands + k0 + gl, q.vocab) : q.vocab;
+    float mine = 0.f;
+    if (q.vocab != 0) {
+      LmRowSum<V, NV, FULL> hr;
+      if constexpr (!BLOCKS) {
+        LmRowPart<T, V, G, NV, FULL> a;
+        a.load(h + (i64)t * q.hStride, 0, gl, shape);
+        a.mask(0, gl, shape);
+        hr.zero();
+        hr.template add<T, G>(1.f, a);
+      }
+      // (an id that names no word reads row 0 for nothing)
+      const u64 atL = rowL < q.vocab ? (u64)rowL * (u64)q.tableStride : 0u;
+      const u32 most = uni(wave_max_u32(cnt));
+      for (u32 k = 0; k < most; k += U) {
+        LmRowPart<T, V, G, NV, FULL> b[U];
+        u64 at[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const u32 k = k0 + (u32)u * kGroups + grp;
-          row[u] = wave_shfl_u32(rowL, (int)(k & 63));
-          if (k >= kn) row[u] = q.vocab;
-          // (a candidate that names no word reads the target's row and leaves with g = 0)
-          if (!BLOCKS) b[u].load(table + (i64)(row[u] < q.vocab ? row[u] : target) * q.tableStride, 0, gl, shape);
+          // (k + u < 16 <= G: kLmScoreCands and U are powers of two)
+          at[u] = wave_shfl_u64(atL, (int)((lane & ~(G - 1)) + k + (u32)u));
+          if constexpr (!BLOCKS) b[u].load(table + at[u], 0, gl, shape);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const u32 k = k0 + (u32)u * kGroups + grp;
-          const bool ok = row[u] < q.vocab;
-          float dot = 0.f;
-          if constexpr (BLOCKS) {
-            for (u32 p0 = 0; ok && p0 < shape.packs; p0 += G * NV) {
-              LmRowPart<T, V, G, NV> a;
-              a.load(h + (i64)t * q.hStride, p0, gl, shape);
-              b[u].load(table + (i64)row[u] * q.tableStride, p0, gl, shape);
-              LmRowSum<V, NV> x;
-              x.zero();
-              x.template add<T, G>(1.f, a);
-              dot += x.template dot<T, G>(b[u]);
+          if (k + (u32)u < most) {
+            float dot;
+            if constexpr (BLOCKS) {
+              dot = lm_dot_blocks<T, V, G, NV>(h + (i64)t * q.hStride, table + at[u], gl, shape);
+            } else {
+              b[u].mask(0, gl, shape);
+              dot = hr.template dot<T, G>(b[u]);
             }
+            dot = lm_group_sum<G>(dot);
+            if (gl == k + (u32)u) mine = dot;
+          }
+        }
+      }
+    }
+    if (gl < cnt) q.out[t * q.cands + k0 + gl] = rowL < q.vocab ? mine - q.constant : -__builtin_inff();
+  }
+}
+
+// A wavefront a token, its groups side by side over the candidates.  What the next token needs is requested while this one's
+// rows are on their way: its ids first, then, from them, the logarithms of its noise, and its row of h.
+template <class T, int V, int G, int NV, LmRowKind KIND, bool DH>
+__global__ void __launch_bounds__(kLmThreads)
+    k_lm_nce_loss(LmNce q, const typename T::store* __restrict__ h, const typename T::store* __restrict__ table, LmIds ids,
+                  typename T::store* __restrict__ dh) {
+  constexpr bool BLOCKS = KIND == kLmBlocks, FULL = KIND == kLmFull;
+  constexpr u32 kGroups = 64 / G;
+  constexpr int U = BLOCKS ? 1 : lm_rows_in_flight<T, V, NV>() / 2;
+  const int lane = (int)(threadIdx.x & 63);
+  const u32 gl = threadIdx.x & (G - 1), grp = (u32)lane / G;
+  const LmRowShape shape = {q.dim / V, q.dim % V};
+  const u64 step = (u64)gridDim.x * (kLmThreads / 64);
+  const u64 t00 = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6);
+  const u32 ahead = q.cands < 64 ? q.cands : 64u;
+  u32 rowN = q.vocab;
+  float lnN = 0.f;
+  LmRowPart<T, V, G, NV, FULL> hN;
+  auto fetch_ids = [&](u64 t) {
+    rowN = q.vocab;
+    if (t < q.n && (u32)lane < ahead) rowN = lm_row(ids, t * q.cands + (u32)lane, q.vocab);
+  };
+  auto fetch_rest = [&](u64 t) {
+    lnN = 0.f;
+    if (rowN < q.vocab) lnN = q.logNoise[rowN];
+    if constexpr (!BLOCKS) hN.load(h + (i64)(t < q.n ? t : t00) * q.hStride, 0, gl, shape);
+  };
+  if (t00 >= q.n) return;
+  fetch_ids(t00);
+  fetch_rest(t00);
+  for (u64 t = t00; t < q.n; t += step) {
+    u32 rowL = rowN;
+    float lnL = lnN;
+    const u32 target = wave_bcast_u32(rowL, 0);
+    const bool live = target < q.vocab;
+    const float w = q.weight != nullptr ? q.weight[t] : 1.f;
+    LmRowSum<V, NV, FULL> hr, acc;
+    hr.zero();
+    acc.zero();
+    float loss = 0.f;
+    if constexpr (!BLOCKS) {
+      hN.mask(0, gl, shape);
+      hr.template add<T, G>(1.f, hN);
+    }
+    fetch_ids(t + step);
+    if (!live) fetch_rest(t + step);
+    for (u32 kb = 0; live && kb < q.cands; kb += 64) {
+      const u32 kn = q.cands - kb < 64 ? q.cands - kb : 64u;
+      if (kb > 0) {
+        rowL = (u32)lane < kn ? lm_row(ids, t * q.cands + kb + (u32)lane, q.vocab) : q.vocab;
+        lnL = rowL < q.vocab ? q.logNoise[rowL] : 0.f;
+      }
+      const float biasL = q.constant + lnL;
+      // (a candidate that names no word reads the target's row and leaves with a gradient of zero)
+      const u64 atL = (u64)(rowL < q.vocab ? rowL : target) * (u64)q.tableStride;
+      const u64 okL64 = wave_ballot(rowL < q.vocab);
+      // lane k keeps what is candidate k's alone: its logit now, its loss and gradient once for all 64 behind the loop.  In
+      // the loop a group makes the gradient of its candidate only as far as dh needs it.
+      float zL = 0.f;
+      for (u32 k0 = 0; k0 < kn; k0 += kGroups * U) {
+        LmRowPart<T, V, G, NV, FULL> b[U];
+        u64 at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          at[u] = wave_shfl_u64(atL, (int)((k0 + (u32)u * kGroups + grp) & 63));
+          if (!BLOCKS) b[u].load(table + at[u], 0, gl, shape);
+        }
+        if (kb + k0 == 0) fetch_rest(t + step);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const u32 k = k0 + (u32)u * kGroups + grp;
+          if (k0 + (u32)u * kGroups >= kn) continue;
+          const bool ok = k < kn && ((okL64 >> (k & 63)) & 1) != 0;
+          float dot;
+          if constexpr (BLOCKS) {
+            dot = lm_dot_blocks<T, V, G, NV>(h + (i64)t * q.hStride, table + at[u], gl, shape);
           } else {
+            b[u].mask(0, gl, shape);
             dot = hr.template dot<T, G>(b[u]);
           }
           dot = lm_group_sum<G>(dot);
           const float z = dot - wave_shfl_f32(biasL, (int)(k & 63));
-          const float sign = kb + k == 0 ? -1.f : 1.f;
-          float sg;
-          const float l = lm_softplus(sign * z, sg);
-          loss += ok ? l : 0.f;
-          const float g = ok ? sign * sg * w : 0.f;
-          // lane k keeps candidate k's gradient: group k mod kGroups holds it now
-          const float mine = wave_shfl_f32(g, (int)(((u32)lane & (kGroups - 1)) * G));
+          // (lane k of the 64 reads group k mod kGroups)
+          const float mine = kGroups == 1 ? z : wave_shfl_f32(z, (int)(((u32)lane & (kGroups - 1)) * G));
           const u32 k1 = k0 + (u32)u * kGroups;
-          if ((u32)lane >= k1 && (u32)lane < k1 + kGroups) gL = mine;
-          if (DH && !BLOCKS && ok) acc.template add<T, G>(g, b[u]);
+          if ((u32)lane >= k1 && (u32)lane < k1 + kGroups) zL = mine;
+          if (DH && !BLOCKS) {
+            float a, c;
+            lm_gate(kb + k == 0 ? -z : z, a, c);
+            if (ok) acc.template add<T, G>(kb + k == 0 ? -a * w : a * w, b[u]);
+          }
         }
       }
-      if (q.g != nullptr && (u32)lane < kn) q.g[t * q.cands + kb + (u32)lane] = gL;
+      const float sign = kb + (u32)lane == 0 ? -1.f : 1.f;
+      float sg;
+      const float l = lm_softplus(sign * zL, sg);
+      const bool okL = rowL < q.vocab;
+      loss += okL ? l : 0.f;
+      if (q.g != nullptr && (u32)lane < kn) q.g[t * q.cands + kb + (u32)lane] = okL ? sign * sg * w : 0.f;
     }
     if constexpr (BLOCKS) {
       if (DH) {
@@ -207,8 +310,9 @@ __global__ void __launch_bounds__(kLmThreads)
           for (u32 k = 0; live && k < q.cands; ++k) {
             const u32 r = uni(lm_row(ids, t * q.cands + k, q.vocab));
             if (r == q.vocab) continue;
-            LmRowPart<T, V, G, NV> b;
+            LmRowPart<T, V, G, NV, FULL> b;
             b.load(table + (i64)r * q.tableStride, p0, gl, shape);
+            b.mask(p0, gl, shape);
             acc.template add<T, G>(q.g[t * q.cands + k], b);
           }
           acc.template store<T, G>(dh + (i64)t * q.dhStride, p0, gl, shape);
@@ -218,7 +322,6 @@ __global__ void __launch_bounds__(kLmThreads)
       // the groups' parts, in a fixed tree
 #pragma unroll
       for (int d = G; d < 64; d *= 2) {
-        loss += wave_shfl_f32(loss, lane ^ d);
         if (DH) {
 #pragma unroll
           for (int i = 0; i < NV; ++i)
@@ -229,6 +332,7 @@ __global__ void __launch_bounds__(kLmThreads)
       }
       if (DH && grp == 0) acc.template store<T, G>(dh + (i64)t * q.dhStride, 0, gl, shape);
     }
+    loss = lm_group_sum<64>(loss);
     if (lane == 0) q.out[t] = live ? loss * w : 0.f;
   }
 }

@@ -82,7 +82,7 @@ __device__ __forceinline__ void lm_row_f32(const float* base, i64 stride, u32 ro
   }
   const LmPack<LmF32, V> p = lm_load<LmF32, V>(base + (i64)row * stride + col);
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = p.v[e];
+  for (int e = 0; e < V; ++e) v[e] = p.get(e);
 }
 template <int V>
 __device__ __forceinline__ void lm_put_f32(float* base, i64 stride, u32 row, u32 col, const float (&v)[V]) {
@@ -90,7 +90,7 @@ __device__ __forceinline__ void lm_put_f32(float* base, i64 stride, u32 row, u32
 }
 
 // Rows [r0, r1) of one sentence, forward, from state v.
-template <class T, int V, bool SAVE>
+template <class T, int V, bool SAVE, bool STREAM>
 __device__ __forceinline__ void lm_scan_rows(const LmScan<T>& q, u32 r0, u32 r1, u32 col, float (&v)[V]) {
   for (u32 t = r0; t < r1;) {
     const u32 cut = (t / kLmSave + 1) * kLmSave;
@@ -109,10 +109,10 @@ __device__ __forceinline__ void lm_scan_rows(const LmScan<T>& q, u32 r0, u32 r1,
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           float a, b;
-          lm_gate(T::get(f[i].v[e]), a, b);
-          v[e] = __builtin_fmaf(a, v[e], b * T::get(x[i].v[e]));
+          lm_gate(f[i].get(e), a, b);
+          v[e] = __builtin_fmaf(a, v[e], b * x[i].get(e));
         }
-        lm_store<T, V>(q.h + (i64)(t + i) * q.hStride + col, lm_pack<T, V>(v));
+        lm_store<T, V, STREAM>(q.h + (i64)(t + i) * q.hStride + col, lm_pack<T, V>(v));
       }
     }
     t += cnt;
@@ -121,7 +121,7 @@ __device__ __forceinline__ void lm_scan_rows(const LmScan<T>& q, u32 r0, u32 r1,
 
 // Rows [r0, r1) of a sentence that begins at row `begin`, backward; e: gradient of the state behind row r1 - 1 on entry, of
 // the state in front of row r0 on return.
-template <class T, int V>
+template <class T, int V, bool STREAM>
 __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 sentence, u32 begin, u32 r0, u32 r1, u32 col, float (&e)[V]) {
   for (u32 end = r1; end > r0;) {
     const u32 cut = (end - 1) / kLmSave * kLmSave;
@@ -143,9 +143,9 @@ __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 senten
     for (u32 i = 0; i < kLmSave; ++i) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        lm_gate(T::get(f[i].v[k]), a[i][k], b[i][k]);
+        lm_gate(f[i].get(k), a[i][k], b[i][k]);
         before[i][k] = v[k];
-        v[k] = __builtin_fmaf(a[i][k], v[k], b[i][k] * T::get(x[i].v[k]));
+        v[k] = __builtin_fmaf(a[i][k], v[k], b[i][k] * x[i].get(k));
       }
     }
 #pragma unroll
@@ -155,13 +155,13 @@ __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 senten
         float df[V], dx[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float delta = T::get(d[i].v[k]) + e[k];
+          const float delta = d[i].get(k) + e[k];
           dx[k] = delta * b[i][k];
           e[k] = delta * a[i][k];
-          df[k] = dx[k] * (before[i][k] - T::get(x[i].v[k])) * a[i][k];
+          df[k] = dx[k] * (before[i][k] - x[i].get(k)) * a[i][k];
         }
-        lm_store<T, V>(q.dgate + (i64)(t + i) * q.dgateStride + col, lm_pack<T, V>(df));
-        lm_store<T, V>(q.dx + (i64)(t + i) * q.dxStride + col, lm_pack<T, V>(dx));
+        lm_store<T, V, STREAM>(q.dgate + (i64)(t + i) * q.dgateStride + col, lm_pack<T, V>(df));
+        lm_store<T, V, STREAM>(q.dx + (i64)(t + i) * q.dxStride + col, lm_pack<T, V>(dx));
       }
     }
     end = t;
@@ -169,7 +169,7 @@ __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 senten
 }
 
 // ---- a wavefront per sentence and column block -----------------------------------
-template <class T, int V, bool SAVE>
+template <class T, int V, bool SAVE, bool STREAM>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_seq(LmScan<T> q) {
   const u64 tasks = (u64)q.n * q.colBlocks;
   for (u64 task = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6); task < tasks; task += (u64)gridDim.x * (kLmThreads / 64)) {
@@ -180,12 +180,12 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_seq(LmScan<T> q) {
     const u32 r0 = lm_offset(q.offsets, i, q.rows), r1 = lm_offset(q.offsets, i + 1, q.rows);
     float v[V];
     lm_row_f32<V>(q.state, q.stateStride, i, col, v);
-    if (r0 < r1) lm_scan_rows<T, V, SAVE>(q, r0, r1, col, v);
+    if (r0 < r1) lm_scan_rows<T, V, SAVE, STREAM>(q, r0, r1, col, v);
     if (q.last != nullptr) lm_put_f32<V>(q.last, q.lastStride, i, col, v);
   }
 }
 
-template <class T, int V>
+template <class T, int V, bool STREAM>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_seq(LmScan<T> q) {
   const u64 tasks = (u64)q.n * q.colBlocks;
   for (u64 task = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6); task < tasks; task += (u64)gridDim.x * (kLmThreads / 64)) {
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_seq(LmScan<T> q) {
     const u32 r0 = lm_offset(q.offsets, i, q.rows), r1 = lm_offset(q.offsets, i + 1, q.rows);
     float e[V];
     lm_row_f32<V>(q.dlast, q.dlastStride, i, col, e);
-    if (r0 < r1) lm_scan_grad_rows<T, V>(q, i, r0, r0, r1, col, e);
+    if (r0 < r1) lm_scan_grad_rows<T, V, STREAM>(q, i, r0, r0, r1, col, e);
     if (q.dstate != nullptr) lm_put_f32<V>(q.dstate, q.dstateStride, i, col, e);
   }
 }
@@ -244,9 +244,9 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_agg(LmScan<T> q) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             float a, b;
-            lm_gate(T::get(f[k].v[e]), a, b);
+            lm_gate(f[k].get(e), a, b);
             A[e] *= a;
-            B[e] = __builtin_fmaf(a, B[e], b * T::get(x[k].v[e]));
+            B[e] = __builtin_fmaf(a, B[e], b * x[k].get(e));
           }
         }
       }
@@ -301,9 +301,9 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             float a, b;
-            lm_gate(T::get(f[k].v[e]), a, b);
+            lm_gate(f[k].get(e), a, b);
             A[e] *= a;
-            B[e] = a * (B[e] + T::get(d[k].v[e]));
+            B[e] = a * (B[e] + d[k].get(e));
           }
         }
       }
@@ -382,7 +382,7 @@ __device__ __forceinline__ void lm_scan_empty(const i32* offsets, u32 n, u32 row
   }
 }
 
-template <class T, int V, bool SAVE>
+template <class T, int V, bool SAVE, bool STREAM>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_chunk(LmScan<T> q) {
   const u64 tasks = (u64)q.chunks * q.colBlocks;
   for (u64 task = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6); task < tasks; task += (u64)gridDim.x * (kLmThreads / 64)) {
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_chunk(LmScan<T> q) {
       if (begin >= r0) lm_row_f32<V>(q.state, q.stateStride, i, col, v);
       else lm_row_f32<V>(q.aggB, q.dim, c, col, v);
       const u32 to = end < r1 ? end : r1;
-      lm_scan_rows<T, V, SAVE>(q, t, to, col, v);
+      lm_scan_rows<T, V, SAVE, STREAM>(q, t, to, col, v);
       if (to == end && q.last != nullptr) lm_put_f32<V>(q.last, q.lastStride, i, col, v);
       t = to;
       if (t == r1) break;
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_chunk(LmScan<T> q) {
   lm_scan_empty<V>(q.offsets, q.n, q.rows, q.dim, q.colBlocks, q.state, q.stateStride, q.last, q.lastStride);
 }
 
-template <class T, int V>
+template <class T, int V, bool STREAM>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_chunk(LmScan<T> q) {
   const u64 tasks = (u64)q.chunks * q.colBlocks;
   for (u64 task = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6); task < tasks; task += (u64)gridDim.x * (kLmThreads / 64)) {
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_chunk(LmScan<T> q) 
         float e[V];
         if (end <= r1) lm_row_f32<V>(q.dlast, q.dlastStride, i, col, e);
         else lm_row_f32<V>(q.aggB, q.dim, c, col, e);
-        lm_scan_grad_rows<T, V>(q, i, begin, from, to, col, e);
+        lm_scan_grad_rows<T, V, STREAM>(q, i, begin, from, to, col, e);
         if (from == begin && q.dstate != nullptr) lm_put_f32<V>(q.dstate, q.dstateStride, i, col, e);
         t = from;
       }

@@ -16,12 +16,16 @@ There is no CPU implementation behind this module.  (tests/ pass `lib_path` of t
 """
 import ctypes as C
 import struct
+import threading
 
 import torch
 
 from .native import JppGpuError, load_library
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ID_BYTES = {torch.int32: 4, torch.int64: 8}
+_pack_matrix = struct.Struct('=QqiI').pack
+_pack_ids = struct.Struct('=QiI').pack
 _libs = {}
 
 
@@ -46,8 +50,14 @@ def _lib(path=None):
     return lib
 
 
+def _raw_stream(index):
+    """the current stream's handle (torch.cuda.current_stream builds a Stream object around it first: a microsecond)"""
+    get = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def _check(lib, rc):
-    if rc != 0:
+    if rc:
         raise JppGpuError(lib.jppgpu_last_error().decode())
 
 
@@ -57,40 +67,47 @@ def _refuse(why):
 
 def _where(lib_path, first, *others):
     """(device ordinal, stream) of the call; every tensor on the device of the first"""
-    dev = first.device
+    index = first.get_device()
     for t in others:
-        if t is not None and t.device != dev:
-            _refuse('the tensors are on different devices (%s, %s)' % (dev, t.device))
-    if dev.type != 'cuda':
-        if lib_path is None or dev.type != 'cpu':
-            _refuse('the tensors are on %s, not on a GPU' % dev)
+        if t is not None and t.get_device() != index:
+            _refuse('the tensors are on different devices (%s, %s)' % (first.device, t.device))
+    if index < 0:
+        if lib_path is None or first.device.type != 'cpu':
+            _refuse('the tensors are on %s, not on a GPU' % first.device)
         return 0, None   # (device memory of the emulator build is host memory)
-    return dev.index, torch.cuda.current_stream(dev).cuda_stream
+    return index, _raw_stream(index)
 
 
-def _rows(t, what, shape=None):
-    """the packed jppgpu_lm_matrix of a 2-d tensor"""
-    code = _TYPES.get(t.dtype)
-    if code is None:
-        _refuse('%s is %s; float32, bfloat16 and float16 are supported' % (what, t.dtype))
-    if t.dim() != 2:
+def _rows(t, what, n=None, dim=None):
+    """the packed jppgpu_lm_matrix of a 2-d tensor (of n x dim, where given)"""
+    try:
+        rows, cols = t.shape
+        stride, step = t.stride()
+        code = _TYPES[t.dtype]
+    except ValueError:
         _refuse('%s has %d dimensions, not 2' % (what, t.dim()))
-    if shape is not None and tuple(t.shape) != shape:
-        _refuse('%s is %s, not %s' % (what, tuple(t.shape), shape))
-    n, d = t.shape
-    if d > 1 and t.stride(1) != 1:
+    except KeyError:
+        _refuse('%s is %s; float32, bfloat16 and float16 are supported' % (what, t.dtype))
+    if n is not None and (rows != n or cols != dim):
+        _refuse('%s is %s, not (%d, %d)' % (what, tuple(t.shape), n, dim))
+    if step != 1 and cols > 1:
         _refuse('the columns of %s are not contiguous' % what)
     # (torch gives a tensor of at most one row any stride)
-    stride = t.stride(0) if n > 1 else d
-    return struct.pack('=QqiI', t.data_ptr(), stride, code, 0)
+    return _pack_matrix(t.data_ptr(), stride if rows > 1 else cols, code, 0)
+
+
+def _out(t, dim):
+    """... of one of our own results"""
+    return _pack_matrix(t.data_ptr(), dim, _TYPES[t.dtype], 0)
 
 
 def _ids(t, what='ids'):
-    if t.dtype not in (torch.int32, torch.int64):
+    size = _ID_BYTES.get(t.dtype)
+    if size is None:
         _refuse('%s are %s, not int32 or int64' % (what, t.dtype))
     if not t.is_contiguous():
         _refuse('%s are not contiguous' % what)
-    return struct.pack('=QiI', t.data_ptr(), 4 if t.dtype == torch.int32 else 8, 0)
+    return _pack_ids(t.data_ptr(), size, 0)
 
 
 def _vector(t, what, n, dtype):
@@ -99,9 +116,18 @@ def _vector(t, what, n, dtype):
     return t.data_ptr()
 
 
+_need = threading.local()
+
+
 def _workspace(lib, fn, args, device):
-    need = C.c_uint64()
-    _check(lib, fn(*args, C.addressof(need)))
+    """(tensor or None, pointer, bytes) of a workspace; torch's allocator keeps it for the stream, or for the graph"""
+    try:
+        need, at = _need.value
+    except AttributeError:
+        need = C.c_uint64()
+        at = C.addressof(need)
+        _need.value = need, at
+    _check(lib, fn(*args, at))
     if need.value == 0:
         return None, 0, 0
     ws = torch.empty(need.value, dtype=torch.uint8, device=device)
@@ -118,7 +144,7 @@ def embed(table, ids, scale=1.0, dtype=None, lib_path=None):
     rows, idv = _rows(table, 'table'), _ids(ids)
     n, (vocab, dim) = ids.shape[0], table.shape
     out = torch.empty((n, dim), dtype=dtype or table.dtype, device=table.device)
-    _check(lib, lib.jppgpu_lm_embed(rows, vocab, dim, idv, n, scale, _rows(out, 'the result'), dev, stream))
+    _check(lib, lib.jppgpu_lm_embed(rows, vocab, dim, idv, n, scale, _out(out, dim), dev, stream))
     return out
 
 
@@ -132,7 +158,7 @@ def embed_grad(dy, ids, vocab, scale=1.0, lib_path=None):
     n, dim = dy.shape
     ws, wp, wn = _workspace(lib, lib.jppgpu_lm_embed_grad_workspace, (n, vocab, dim), dy.device)
     grad = torch.empty((vocab, dim), dtype=torch.float32, device=dy.device)
-    _check(lib, lib.jppgpu_lm_embed_grad(rows, idv, n, vocab, dim, scale, _rows(grad, 'the gradient'), wp, wn, dev, stream))
+    _check(lib, lib.jppgpu_lm_embed_grad(rows, idv, n, vocab, dim, scale, _out(grad, dim), wp, wn, dev, stream))
     return grad
 
 
@@ -155,15 +181,15 @@ def scan(gate, x, offsets=None, state=None, max_len=None, save=False, lib_path=N
     dev, stream = _where(lib_path, x, gate, offsets, state)
     xv = _rows(x, 'x')
     rows, dim = x.shape
-    gv = _rows(gate, 'gate', (rows, dim))
+    gv = _rows(gate, 'gate', rows, dim)
     offsets, op, n = _batch(offsets, rows, x.device)
-    sv = _rows(state, 'state', (n, dim)) if state is not None else None
+    sv = _rows(state, 'state', n, dim) if state is not None else None
     max_len = max_len or 0
     h = torch.empty((rows, dim), dtype=x.dtype, device=x.device)
     last = torch.empty((n, dim), dtype=torch.float32, device=x.device)
     saved = torch.empty((lib.jppgpu_lm_scan_saved(rows), dim), dtype=torch.float32, device=x.device) if save else None
     ws, wp, wn = _workspace(lib, lib.jppgpu_lm_scan_workspace, (rows, n, dim, max_len), x.device)
-    _check(lib, lib.jppgpu_lm_scan(gv, xv, op, n, rows, dim, max_len, sv, _rows(h, 'h'), _rows(last, 'last'),
+    _check(lib, lib.jppgpu_lm_scan(gv, xv, op, n, rows, dim, max_len, sv, _out(h, dim), _out(last, dim),
                                    saved.data_ptr() if save else None, wp, wn, dev, stream))
     return (h, last, saved) if save else (h, last)
 
@@ -175,18 +201,18 @@ def scan_grad(gate, x, dh, saved, offsets=None, state=None, dlast=None, max_len=
     dev, stream = _where(lib_path, x, gate, dh, saved, offsets, state, dlast)
     xv = _rows(x, 'x')
     rows, dim = x.shape
-    gv, dv = _rows(gate, 'gate', (rows, dim)), _rows(dh, 'dh', (rows, dim))
+    gv, dv = _rows(gate, 'gate', rows, dim), _rows(dh, 'dh', rows, dim)
     offsets, op, n = _batch(offsets, rows, x.device)
-    sv = _rows(state, 'state', (n, dim)) if state is not None else None
-    lv = _rows(dlast, 'dlast', (n, dim)) if dlast is not None else None
+    sv = _rows(state, 'state', n, dim) if state is not None else None
+    lv = _rows(dlast, 'dlast', n, dim) if dlast is not None else None
     if saved.dtype != torch.float32 or tuple(saved.shape) != (lib.jppgpu_lm_scan_saved(rows), dim) or not saved.is_contiguous():
         _refuse('saved is not what scan(..., save=True) returned for these rows')
     max_len = max_len or 0
     dgate, dx = (torch.empty((rows, dim), dtype=x.dtype, device=x.device) for _ in range(2))
     dstate = torch.empty((n, dim), dtype=torch.float32, device=x.device)
     ws, wp, wn = _workspace(lib, lib.jppgpu_lm_scan_workspace, (rows, n, dim, max_len), x.device)
-    _check(lib, lib.jppgpu_lm_scan_grad(gv, xv, op, n, rows, dim, max_len, sv, saved.data_ptr(), dv, lv, _rows(dgate, 'dgate'),
-                                        _rows(dx, 'dx'), _rows(dstate, 'dstate'), wp, wn, dev, stream))
+    _check(lib, lib.jppgpu_lm_scan_grad(gv, xv, op, n, rows, dim, max_len, sv, saved.data_ptr(), dv, lv, _out(dgate, dim),
+                                        _out(dx, dim), _out(dstate, dim), wp, wn, dev, stream))
     return dgate, dx, dstate
 
 
@@ -230,6 +256,6 @@ def nce_loss(h, table, ids, log_noise, constant, weight=None, grads=True, lib_pa
     ws, wp, wn = _workspace(lib, lib.jppgpu_lm_nce_loss_workspace, (n, cands, vocab, dim), h.device)
     dh = torch.empty((n, dim), dtype=h.dtype, device=h.device)
     dtable = torch.empty((vocab, dim), dtype=torch.float32, device=h.device)
-    _check(lib, lib.jppgpu_lm_nce_loss(hv, tv, vocab, dim, idv, n, cands, ln, constant, wt, loss.data_ptr(), _rows(dh, 'dh'),
-                                       _rows(dtable, 'dtable'), wp, wn, dev, stream))
+    _check(lib, lib.jppgpu_lm_nce_loss(hv, tv, vocab, dim, idv, n, cands, ln, constant, wt, loss.data_ptr(), _out(dh, dim),
+                                       _out(dtable, dim), wp, wn, dev, stream))
     return loss, dh, dtable
