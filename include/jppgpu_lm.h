@@ -12,7 +12,7 @@
  * Threads may call at once; the caller owns the workspaces, and two calls that may run at once need two.  Results do not
  * depend on timing: the same inputs give the same bits.
  *
- * Matrices are rows with a stride (in elements, at least the row length) and contiguous columns, of 32-bit floats, bfloat16
+ * Matrices are rows with a stride (in elements, at least the row length, below 2^32) and contiguous columns, of 32-bit floats, bfloat16
  * or IEEE half.  Sums, states and softplus are held in 32 bits, an output is rounded once.  Outputs must not overlap inputs
  * or each other.  Word ids are int32 or int64; one outside [0, vocab) names no word.
  *

@@ -246,6 +246,34 @@ __device__ __forceinline__ float lm_group_sum(float v) {
 #endif
 }
 
+// Sums over the four rows of 16 lanes, the rows sharing the result: of v[0 .. N - 1] in every row, row r keeps the N / 4
+// sums of elements r N / 4 .. in v[0 .. N / 4 - 1].  Lanes 32 apart swap halves of the array, then lanes 16 apart.
+template <int N>
+__device__ __forceinline__ void lm_rows_share(float (&v)[N]) {
+  static_assert(N % 4 == 0, "a quarter each");
+  auto exchange = [&](float& a, float& b, auto half) {   // a: the sum over the pair in the lower lanes, b's in the upper
+#if defined(__HIP_DEVICE_COMPILE__)
+    const u32 x = __builtin_bit_cast(u32, a), y = __builtin_bit_cast(u32, b);
+    if constexpr (decltype(half)::value == 32) {
+      const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+      a = __builtin_bit_cast(float, r[0]) + __builtin_bit_cast(float, r[1]);
+    } else {
+      const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+      a = __builtin_bit_cast(float, r[0]) + __builtin_bit_cast(float, r[1]);
+    }
+#else
+    constexpr int d = decltype(half)::value;
+    const bool up = (lane_id() & d) != 0;
+    const float mine = up ? b : a, other = wave_shfl_f32(up ? a : b, lane_id() ^ d);
+    a = up ? other + mine : mine + other;
+#endif
+  };
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) exchange(v[i], v[i + N / 2], LmConst<32>());
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) exchange(v[i], v[i + N / 4], LmConst<16>());
+}
+
 // ---- ids -----------------------------------------------------------------------
 struct LmIds {
   const void* data;
@@ -256,6 +284,18 @@ __device__ __forceinline__ u32 lm_row(const LmIds& ids, u64 i, u32 vocab) {
   const i64 v = ids.wide ? as_global(static_cast<const i64*>(ids.data))[i] : (i64)as_global(static_cast<const i32*>(ids.data))[i];
   return v >= 0 && v < (i64)vocab ? (u32)v : vocab;
 }
+
+// j / d for 0 <= j < 2^31, 1 <= d < 2^31, by a product: m = ceil(2^(31 + s) / d) with 2^s >= d, so the error of j m / 2^(31 + s)
+// stays below 1 / d
+struct LmDiv {
+  u32 mul, shift;
+  static LmDiv by(u32 d) {
+    u32 s = 0;
+    while ((u64{1} << s) < d) ++s;
+    return LmDiv{(u32)(((u64{1} << (31 + s)) + d - 1) / d), 31 + s};
+  }
+  __device__ __forceinline__ u32 operator()(u32 j) const { return (u32)((u64)j * mul >> shift); }
+};
 
 constexpr u32 kLmThreads = 256;        // threads of a workgroup, where a kernel has no reason for another number
 constexpr u64 kLmChipBlocks = 256 * 8; // workgroups of kLmThreads threads that the 256 compute units hold at most

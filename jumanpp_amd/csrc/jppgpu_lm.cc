@@ -91,7 +91,7 @@ bool streamed(u64 bytes) { return bytes > kStreamBytes; }
 u64 div_up(u64 a, u64 b) { return (a + b - 1) / b; }
 
 // ---- checks --------------------------------------------------------------------------
-constexpr int64_t kMaxDim = 1 << 24, kMaxRows = int64_t{1} << 40, kMaxStride = int64_t{1} << 40;
+constexpr int64_t kMaxDim = 1 << 24, kMaxRows = int64_t{1} << 40, kMaxStride = 0xffffffff;
 constexpr int64_t kMaxIndex = 0x7fffffff;   // words, packed rows, sentences, entries of a sum by word
 
 int bytes_of(int32_t type) { return type == JPPGPU_LM_F32 ? 4 : 2; }
@@ -105,7 +105,7 @@ const char* bad_matrix(const jppgpu_lm_matrix* m, int64_t rows, int64_t dim, Nee
   if (m->type != JPPGPU_LM_F32 && m->type != JPPGPU_LM_BF16 && m->type != JPPGPU_LM_F16) return "unknown element type";
   if (m->data == nullptr) return need == kOptional || rows == 0 ? nullptr : "a matrix has no data";
   if (reinterpret_cast<uintptr_t>(m->data) % (uintptr_t)bytes_of(m->type) != 0) return "a matrix does not start on an element";
-  if (m->stride < dim || m->stride > kMaxStride) return "the stride of a matrix is shorter than its rows, or beyond 2^40";
+  if (m->stride < dim || m->stride > kMaxStride) return "the stride of a matrix is shorter than its rows, or beyond 2^32 - 1";
   return nullptr;
 }
 
@@ -162,39 +162,48 @@ int bad_workspace(const void* p, uint64_t bytes, uint64_t need) {
 }
 
 // ---- sums by word --------------------------------------------------------------------
-// Columns of a wavefront of k_lm_seg_sum: the fewest that leave no second column block up to 256 (a lane's pack is then as
-// small as it can be, and the lanes of a short row are not idle).
-u32 seg_pack(u32 dim) { return dim <= 64 ? 1u : dim <= 128 ? 2u : 4u; }
+constexpr u64 kL2Bytes = u64{4} << 20;   // of an XCD
 
 struct SumPlan {
-  u32 n, dim, keyBits, passes, sortTiles, segTile, segTiles, colBlocks;
-  bool one;
-  LmPair *a, *b;
+  u32 n, dim, keyBits, passes, sortRounds, sortTiles, pack, lanes, part, tile, tiles, colBlocks;
+  bool one, weighted;
+  char *a, *b;           // entries
   u32 *counts, *totals, *spanCount, *span;
   float *head, *tail;
 
-  SumPlan(u64 n_, u64 vocab, u64 dim_) : n((u32)n_), dim((u32)dim_) {
+  // n entries, `perToken` of them read one row of src.  The tiles, and with them the workspace, follow from the sizes
+  // alone, not from the type of src.
+  SumPlan(u64 n_, u64 vocab, u64 dim_, u64 perToken, bool weighted_, i32 type = JPPGPU_LM_F32) : n((u32)n_), dim((u32)dim_), weighted(weighted_) {
     keyBits = 1;
     while ((vocab >> keyBits) != 0) ++keyBits;   // (keys 0 .. vocab)
     passes = (keyBits + 7) / 8;
     one = n <= kLmSortOne;
-    sortTiles = (u32)div_up(n, kLmSortTile);
-    colBlocks = (u32)div_up(div_up(dim, seg_pack(dim)), 64);
-    // a tile long enough that partial rows are rare, short enough that some eight thousand wavefronts share the work
-    segTile = 8;
-    while (segTile < 64 && (u64)n * colBlocks / (segTile * 2) >= 8192) segTile *= 2;
-    segTiles = (u32)div_up(n, segTile);
+    // entries of a thread: eight, or two as long as that makes no more tiles than a workgroup looks back on by itself
+    // (workgroups of 1 024 threads took half as long again for 2.2 M entries)
+    sortRounds = n <= kLmSortOwn * kLmThreads * 2 ? 2 : 8;
+    sortTiles = (u32)div_up(n, kLmThreads * sortRounds);
+    // rows that are read again and do not fit one L2: cache lines of 128 bytes spread over the XCDs (k_lm_seg_sum)
+    const bool sliced = perToken > 1 && dim >= 64 && n / perToken * dim * 2 > kL2Bytes;
+    pack = dim < 4 ? 1 : sliced && bytes_of(type) == 2 ? 8 : 4;
+    lanes = sliced || dim <= 32 ? 8 : dim <= 64 ? 16 : dim <= 128 ? 32 : 64;
+    colBlocks = (u32)div_up(div_up(dim, pack), lanes);
+    // parts long enough that words rarely cross them, short enough that some eight thousand wavefronts share the work
+    part = 8;
+    while (part < 64 && (u64)n * div_up(dim, 256) / (part * 2) >= 8192) part *= 2;
+    tile = part * (kLmThreads / lanes);
+    tiles = (u32)div_up(n, tile);
   }
   u64 carve(void* ws) {
     Carver c{static_cast<char*>(ws)};
-    a = c.take<LmPair>(n);
-    b = passes > 1 && !one ? c.take<LmPair>(n) : nullptr;
+    const u64 bytes = (u64)n * (weighted ? sizeof(LmEntry) : sizeof(LmPair));
+    a = c.take<char>(bytes);
+    b = passes > 1 && !one ? c.take<char>(bytes) : nullptr;
     counts = one ? nullptr : c.take<u32>((u64)kLmBins * sortTiles);
     totals = one ? nullptr : c.take<u32>(kLmBins);
-    spanCount = c.take<u32>(1);
-    span = c.take<u32>(segTiles);
-    head = c.take<float>((u64)segTiles * dim);
-    tail = c.take<float>((u64)segTiles * dim);
+    spanCount = c.take<u32>(2);
+    span = c.take<u32>(tiles);
+    head = c.take<float>((u64)tiles * dim);
+    tail = c.take<float>((u64)tiles * dim);
     return c.used;
   }
 };
@@ -208,74 +217,101 @@ LmZero zero_of(float* data, i64 stride, u64 rows, u64 cols) {
 }
 u64 zero_blocks(const LmZero& z) { return z.rows < 2048 ? z.rows : 2048; }
 
-template <class T>
-void launch_seg_sum(Launcher& go, const LmSeg& q, const void* src) {
-  const u64 blocks = div_up((u64)q.tiles * q.colBlocks, kLmThreads / 64);
+template <class T, class E>
+void launch_seg_sum(Launcher& go, const LmSeg<E>& q, u32 pack, u32 lanes, const void* src) {
+  const u64 blocks = (u64)q.tiles * q.colBlocks;
   const typename T::store* s = static_cast<const typename T::store*>(src);
-  switch (seg_pack(q.dim)) {
-    case 1: go(k_lm_seg_sum<T, 1>, blocks, kLmThreads, q, s); break;
-    case 2: go(k_lm_seg_sum<T, 2>, blocks, kLmThreads, q, s); break;
-    default: go(k_lm_seg_sum<T, 4>, blocks, kLmThreads, q, s); break;
+  if (pack == 1) {
+    go(k_lm_seg_sum<T, 1, 8, E>, blocks, kLmThreads, q, s);
+    return;
+  }
+  if constexpr (sizeof(typename T::store) == 2 && E::kWeighted) {
+    if (pack == 8) {
+      go(k_lm_seg_sum<T, 8, 8, E>, blocks, kLmThreads, q, s);
+      return;
+    }
+  }
+  switch (lanes) {
+    case 8: go(k_lm_seg_sum<T, 4, 8, E>, blocks, kLmThreads, q, s); break;
+    case 16: go(k_lm_seg_sum<T, 4, 16, E>, blocks, kLmThreads, q, s); break;
+    case 32: go(k_lm_seg_sum<T, 4, 32, E>, blocks, kLmThreads, q, s); break;
+    default: go(k_lm_seg_sum<T, 4, 64, E>, blocks, kLmThreads, q, s); break;
   }
 }
 
-// grad = the sums by word of the weighted rows of src (jppgpu_lm.h); n > 0
-void sum_by_word(Launcher& go, SumPlan& p, const jppgpu_lm_ids* ids, u32 perToken, float scale, const float* weights, const void* src,
-                 i64 srcStride, i32 srcType, u32 vocab, float* grad, i64 gradStride) {
-  const LmZero zero = zero_of(grad, gradStride, vocab, p.dim);
-  const LmKeysOfIds keys{ids_of(ids), vocab, perToken};
+// what sum_by_word sums
+struct SumSource {
+  const jppgpu_lm_ids* ids;
+  u32 vocab, perToken;
+  float scale;
+  const float* weights;   // or null
+  const jppgpu_lm_matrix* src;
+  float* grad;
+  i64 gradStride;
+};
+
+template <class E, class Keys>
+void sort_pass(Launcher& go, const SumPlan& p, const Keys& keys, u32 shift, u32 bits, const LmZero& zero, E* to) {
   const u64 zeroBlocks = zero_blocks(zero);
-  const LmPair* sorted = p.a;
+  const u32 mask = (1u << bits) - 1;
+  if (p.sortRounds == 2) go(k_lm_sort_count<2, Keys>, p.sortTiles + zeroBlocks, kLmThreads, keys, p.n, shift, mask, p.counts, p.sortTiles, p.spanCount, zero);
+  else go(k_lm_sort_count<8, Keys>, p.sortTiles + zeroBlocks, kLmThreads, keys, p.n, shift, mask, p.counts, p.sortTiles, p.spanCount, zero);
+  if (p.sortTiles > kLmSortOwn) go(k_lm_sort_scan, kLmBins, kLmThreads, p.counts, p.sortTiles, p.totals);
+  if (p.sortRounds == 2) go(k_lm_sort_scatter<2, E, Keys>, p.sortTiles, kLmThreads, keys, p.n, shift, bits, p.counts, p.sortTiles, p.totals, to);
+  else go(k_lm_sort_scatter<8, E, Keys>, p.sortTiles, kLmThreads, keys, p.n, shift, bits, p.counts, p.sortTiles, p.totals, to);
+}
+
+template <class E>
+void sum_entries(Launcher& go, SumPlan& p, const SumSource& x) {
+  const LmZero zero = zero_of(x.grad, x.gradStride, x.vocab, p.dim);
+  const LmKeysOfIds<E> keys{ids_of(x.ids), x.vocab, x.perToken, LmDiv::by(x.perToken), x.weights};
+  E *a = reinterpret_cast<E*>(p.a), *b = reinterpret_cast<E*>(p.b), *sorted = a;
   if (p.one) {
-    go(k_lm_sort_one<LmKeysOfIds>, 1 + zeroBlocks, (u32)kLmOneThreads, keys, p.n, p.keyBits, p.passes, p.a, p.spanCount, zero);
+    go(k_lm_sort_one<E>, 1 + zero_blocks(zero), (u32)kLmOneThreads, keys, p.n, p.keyBits, p.passes, a, p.spanCount, zero);
   } else {
     const u32 digit = (p.keyBits + p.passes - 1) / p.passes;
     const LmZero none{nullptr, 0, 0, 0, 0};
-    LmPair *from = nullptr, *to = p.a;
+    E *from = nullptr, *to = a;
     for (u32 pass = 0; pass < p.passes; ++pass) {
       const u32 shift = pass * digit;
-      if (pass == 0)
-        go(k_lm_sort_count<LmKeysOfIds>, p.sortTiles + zeroBlocks, kLmThreads, keys, p.n, shift, (1u << digit) - 1, p.counts, p.sortTiles,
-           p.spanCount, zero);
-      else
-        go(k_lm_sort_count<LmKeysOfPairs>, p.sortTiles, kLmThreads, LmKeysOfPairs{from}, p.n, shift, (1u << digit) - 1, p.counts, p.sortTiles,
-           p.spanCount, none);
-      go(k_lm_sort_scan, kLmBins / (kLmThreads / 64), kLmThreads, p.counts, p.sortTiles, p.totals);
-      if (pass == 0)
-        go(k_lm_sort_scatter<LmKeysOfIds>, p.sortTiles, kLmThreads, keys, p.n, shift, digit, p.counts, p.sortTiles, p.totals, to);
-      else
-        go(k_lm_sort_scatter<LmKeysOfPairs>, p.sortTiles, kLmThreads, LmKeysOfPairs{from}, p.n, shift, digit, p.counts, p.sortTiles, p.totals, to);
+      if (pass == 0) sort_pass(go, p, keys, shift, digit, zero, to);
+      else sort_pass(go, p, LmKeysOfPass<E>{from}, shift, digit, none, to);
       sorted = from = to;
-      to = to == p.a ? p.b : p.a;
+      to = to == a ? b : a;
     }
   }
-  LmSeg q{};
-  q.pairs = sorted;
+  LmSeg<E> q{};
+  q.entries = sorted;
   q.n = p.n;
-  q.tile = p.segTile;
-  q.tiles = p.segTiles;
-  q.vocab = vocab;
+  q.part = p.part;
+  q.tile = p.tile;
+  q.tiles = p.tiles;
+  q.vocab = x.vocab;
   q.dim = p.dim;
   q.colBlocks = p.colBlocks;
-  q.perToken = perToken;
-  q.scale = scale;
-  q.weights = weights;
-  q.srcStride = srcStride;
-  q.grad = grad;
-  q.gradStride = gradStride;
+  q.scale = x.scale;
+  q.srcStride = (u32)x.src->stride;
+  q.grad = x.grad;
+  q.gradStride = x.gradStride;
   q.head = p.head;
   q.tail = p.tail;
   q.span = p.span;
   q.spanCount = p.spanCount;
-  switch (srcType) {
-    case JPPGPU_LM_F32: launch_seg_sum<LmF32>(go, q, src); break;
-    case JPPGPU_LM_BF16: launch_seg_sum<LmBf16>(go, q, src); break;
-    default: launch_seg_sum<LmF16>(go, q, src); break;
+  switch (x.src->type) {
+    case JPPGPU_LM_F32: launch_seg_sum<LmF32, E>(go, q, p.pack, p.lanes, x.src->data); break;
+    case JPPGPU_LM_BF16: launch_seg_sum<LmBf16, E>(go, q, p.pack, p.lanes, x.src->data); break;
+    default: launch_seg_sum<LmF16, E>(go, q, p.pack, p.lanes, x.src->data); break;
   }
-  if (p.segTiles > 1) {
-    const u64 most = (u64)p.segTiles * div_up(p.dim, 64);
-    go(k_lm_seg_join, most < 1024 ? most : 1024, 64u * kLmJoinWaves, q);
+  if (p.tiles > 1) {
+    const u64 most = (u64)p.tiles * div_up(p.dim, 64);
+    go(k_lm_seg_join<E>, most < 2048 ? most : 2048, 64u * kLmJoinWaves, q);
   }
+}
+
+// grad = the sums by word of the weighted rows of src (jppgpu_lm.h); n > 0
+void sum_by_word(Launcher& go, SumPlan& p, const SumSource& x) {
+  if (p.weighted) sum_entries<LmEntry>(go, p, x);
+  else sum_entries<LmPair>(go, p, x);
 }
 
 // the gradient of a table that nothing reads
@@ -510,7 +546,7 @@ uint64_t nce_workspace(int64_t n, int64_t cands, int64_t vocab, int64_t dim) {
   const u64 entries = (u64)n * (u64)cands;
   Carver c{nullptr};
   c.take<float>(entries);
-  SumPlan p(entries, (u64)vocab, (u64)dim);
+  SumPlan p(entries, (u64)vocab, (u64)dim, (u64)cands, true);
   return c.used + p.carve(nullptr);
 }
 
@@ -547,7 +583,7 @@ extern "C" int jppgpu_lm_embed_grad_workspace(int64_t n, int64_t vocab, int64_t 
   JPP_LM_CHECK(n >= 0 && n <= kMaxIndex, "n outside 0 .. 2^31 - 1");
   *bytes = 0;
   if (n > 0) {
-    SumPlan p((u64)n, (u64)vocab, (u64)dim);
+    SumPlan p((u64)n, (u64)vocab, (u64)dim, 1, false);
     *bytes = p.carve(nullptr);
   }
   return JPPGPU_OK;
@@ -571,9 +607,9 @@ extern "C" int jppgpu_lm_embed_grad(const jppgpu_lm_matrix* dy, const jppgpu_lm_
     clear_matrix(go, grad, (u64)vocab, (u64)dim);
     return go.rc;
   }
-  SumPlan p((u64)n, (u64)vocab, (u64)dim);
+  SumPlan p((u64)n, (u64)vocab, (u64)dim, 1, false, dy->type);
   p.carve(workspace);
-  sum_by_word(go, p, ids, 1, scale, nullptr, dy->data, dy->stride, dy->type, (u32)vocab, static_cast<float*>(grad->data), grad->stride);
+  sum_by_word(go, p, SumSource{ids, (u32)vocab, 1, scale, nullptr, dy, static_cast<float*>(grad->data), grad->stride});
   return go.rc;
 }
 
@@ -755,9 +791,9 @@ extern "C" int jppgpu_lm_nce_loss(const jppgpu_lm_matrix* h, const jppgpu_lm_mat
   if (grads) q.g = c.take<float>(entries);
   dispatch_nce(go, q, h, table, ids_of(ids), const_cast<void*>(dhp), true);
   if (given(dtable) && vocab > 0) {
-    SumPlan p(entries, (u64)vocab, (u64)dim);
+    SumPlan p(entries, (u64)vocab, (u64)dim, (u64)cands, true, h->type);
     p.carve(static_cast<char*>(workspace) + c.used);
-    sum_by_word(go, p, ids, (u32)cands, 1.f, q.g, h->data, h->stride, h->type, (u32)vocab, static_cast<float*>(dtable->data), dtable->stride);
+    sum_by_word(go, p, SumSource{ids, (u32)vocab, (u32)cands, 1.f, q.g, h, static_cast<float*>(dtable->data), dtable->stride});
   }
   return go.rc;
 }

@@ -4,10 +4,12 @@
 // src_(j / K) the state of its token.
 //
 // The gradient sums by word without atomics on floats, so its bits follow from the inputs:
-//   k_lm_sort_one / k_lm_sort_count, _scan, _scatter   entries into ascending (word, entry): least digit first, stable
-//   k_lm_seg_sum                                       tiles of M sorted entries, a wavefront each: a word whose entries
-//                                                      lie inside one tile is written at once, one that crosses a border
-//                                                      leaves a partial row per tile
+//   k_lm_sort_one / k_lm_sort_count, _scan, _scatter   entries into ascending (word, entry): least digit first, stable; an
+//                                                      entry takes its row of src and its weight along
+//   k_lm_seg_sum                                       a workgroup takes a tile of sorted entries, a group of lanes a part of
+//                                                      it: a word that lies inside one part is written at once, one that
+//                                                      crosses parts is put together in LDS, one that crosses tiles leaves a
+//                                                      partial row per tile
 //   k_lm_seg_join                                      the partial rows of those words, in tile order
 // Rows of words that do not occur are zeroed by workgroups that ride in the grid of the first sorting kernel: that one uses
 // a fraction of the chip.
@@ -80,30 +82,45 @@ __device__ __forceinline__ void lm_zero_rows(const LmZero& z, u64 first, u64 ste
 
 __global__ void __launch_bounds__(kLmThreads) k_lm_zero(LmZero z) { lm_zero_rows(z, blockIdx.x, gridDim.x); }
 
-struct LmPair {      // an entry on its way through the sort
+// an entry on its way through the sort
+struct LmPair {
   u32 key;           // word, `vocab` for none
-  u32 entry;
+  u32 row;           // of src
+  static constexpr bool kWeighted = false;
+};
+struct LmEntry {
+  u32 key;
+  u32 row;
+  float weight;
+  static constexpr bool kWeighted = true;
 };
 
-// where the first pass finds its keys
+// where the first pass finds its entries
+template <class E>
 struct LmKeysOfIds {
   LmIds ids;
   u32 vocab;
-  u32 perToken;      // entries of a token; the token counts only if its entry 0 names a word
-  __device__ __forceinline__ LmPair operator()(u32 j) const {
-    u32 key = lm_row(ids, j, vocab);
-    if (perToken > 1 && key < vocab && lm_row(ids, j / perToken * perToken, vocab) == vocab) key = vocab;
-    return LmPair{key, j};
+  u32 perToken;      // entries of a token (= of a row of src); the token counts only if its entry 0 names a word
+  LmDiv token;       // ... and the division by it
+  const float* weights;
+  __device__ __forceinline__ u32 key(u32 j) const {
+    u32 k = lm_row(ids, j, vocab);
+    if (perToken > 1 && k < vocab && lm_row(ids, token(j) * perToken, vocab) == vocab) k = vocab;
+    return k;
+  }
+  __device__ __forceinline__ E entry(u32 j) const {
+    if constexpr (E::kWeighted) return E{key(j), token(j), weights[j]};
+    else return E{key(j), j};
   }
 };
-struct LmKeysOfPairs {
-  const LmPair* pairs;
-  __device__ __forceinline__ LmPair operator()(u32 j) const { return pairs[j]; }
+template <class E>
+struct LmKeysOfPass {
+  const E* entries;
+  __device__ __forceinline__ u32 key(u32 j) const { return entries[j].key; }
+  __device__ __forceinline__ E entry(u32 j) const { return entries[j]; }
 };
 
-constexpr u32 kLmBins = 256;
-constexpr int kLmSortRounds = 8;                                   // keys of a thread
-constexpr u32 kLmSortTile = kLmThreads * kLmSortRounds;            // keys of a workgroup
+constexpr u32 kLmBins = 256;   // (= kLmThreads: a digit a thread)
 constexpr int kLmOneThreads = 1024, kLmOneRounds = 4;
 constexpr u32 kLmSortOne = kLmOneThreads * kLmOneRounds;           // up to here one workgroup sorts everything in LDS
 
@@ -153,9 +170,9 @@ __device__ __forceinline__ void lm_scan_bins(u32* v, u32* part, int lane, int wv
 
 // Few entries: one workgroup, every pass in LDS.  A thread's keys are those of its rounds, wavefront after wavefront, so
 // the order (wavefront, round, lane) is the order of the list.
-template <class Keys>
+template <class E>
 __global__ void __launch_bounds__(kLmOneThreads)
-    k_lm_sort_one(Keys keys, u32 n, u32 keyBits, u32 passes, LmPair* __restrict__ out, u32* __restrict__ spanCount, LmZero zero) {
+    k_lm_sort_one(LmKeysOfIds<E> keys, u32 n, u32 keyBits, u32 passes, E* __restrict__ out, u32* __restrict__ spanCount, LmZero zero) {
   constexpr int kWaves = kLmOneThreads / 64;
   __shared__ u32 s_key[kLmSortOne];
   __shared__ u32 s_entry[kLmSortOne];
@@ -167,14 +184,15 @@ __global__ void __launch_bounds__(kLmOneThreads)
     return;
   }
   const int lane = (int)(threadIdx.x & 63), wv = (int)(threadIdx.x >> 6);
-  if (threadIdx.x == 0) *spanCount = 0;
+  if (threadIdx.x < 2) spanCount[threadIdx.x] = 0;
   const u32 rounds = (n + kLmOneThreads - 1) / kLmOneThreads;   // (1 .. kLmOneRounds)
   const u32 pos0 = (u32)wv * 64u * rounds + (u32)lane;
-  LmPair p[kLmOneRounds];
+  u32 key[kLmOneRounds], entry[kLmOneRounds];
 #pragma unroll
   for (u32 r = 0; r < (u32)kLmOneRounds; ++r) {
-    p[r] = LmPair{0, 0};
-    if (r < rounds && pos0 + 64 * r < n) p[r] = keys(pos0 + 64 * r);
+    entry[r] = pos0 + 64 * r;
+    key[r] = 0;
+    if (r < rounds && entry[r] < n) key[r] = keys.key(entry[r]);
   }
   const u32 digitBits = (keyBits + passes - 1) / passes;
   for (u32 pass = 0; pass < passes; ++pass) {
@@ -185,11 +203,12 @@ __global__ void __launch_bounds__(kLmOneThreads)
 #pragma unroll
     for (u32 r = 0; r < (u32)kLmOneRounds; ++r) {
       rank[r] = 0;
-      if (r < rounds) rank[r] = lm_rank_round((p[r].key >> shift) & mask, pos0 + 64 * r < n, digitBits, s_cnt[wv], lane);
+      if (r < rounds) rank[r] = lm_rank_round((key[r] >> shift) & mask, pos0 + 64 * r < n, digitBits, s_cnt[wv], lane);
     }
     __syncthreads();
     if (threadIdx.x < kLmBins) {
       u32 run = 0;
+#pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const u32 x = s_cnt[w][threadIdx.x];
         s_cnt[w][threadIdx.x] = run;
@@ -203,28 +222,34 @@ __global__ void __launch_bounds__(kLmOneThreads)
 #pragma unroll
     for (u32 r = 0; r < (u32)kLmOneRounds; ++r) {
       if (r < rounds && pos0 + 64 * r < n) {
-        const u32 d = (p[r].key >> shift) & mask;
+        const u32 d = (key[r] >> shift) & mask;
         const u32 to = s_bin[d] + s_cnt[wv][d] + rank[r];
         if (last) {
-          out[to] = p[r];
+          out[to] = keys.entry(entry[r]);
         } else {
-          s_key[to] = p[r].key;
-          s_entry[to] = p[r].entry;
+          s_key[to] = key[r];
+          s_entry[to] = entry[r];
         }
       }
     }
     __syncthreads();
     if (!last) {
 #pragma unroll
-      for (u32 r = 0; r < (u32)kLmOneRounds; ++r)
-        if (r < rounds && pos0 + 64 * r < n) p[r] = LmPair{s_key[pos0 + 64 * r], s_entry[pos0 + 64 * r]};
+      for (u32 r = 0; r < (u32)kLmOneRounds; ++r) {
+        if (r < rounds && pos0 + 64 * r < n) {
+          key[r] = s_key[pos0 + 64 * r];
+          entry[r] = s_entry[pos0 + 64 * r];
+        }
+      }
       __syncthreads();
     }
   }
 }
 
-// One pass over many entries: digits per tile ...
-template <class Keys>
+// Many entries, a pass, a tile of R entries a thread a workgroup: the digits of every tile ...  counts: [tile][bin] where the scatter kernel sums them itself (`own`),
+// [bin][tile] for k_lm_sort_scan.
+constexpr u32 kLmSortOwn = 64;   // tiles up to which it does: a launch costs more than 64 rows of 1 KB
+template <int R, class Keys>
 __global__ void __launch_bounds__(kLmThreads)
     k_lm_sort_count(Keys keys, u32 n, u32 shift, u32 mask, u32* __restrict__ counts, u32 tiles, u32* __restrict__ spanCount, LmZero zero) {
   __shared__ u32 s_cnt[kLmBins];
@@ -232,66 +257,99 @@ __global__ void __launch_bounds__(kLmThreads)
     lm_zero_rows(zero, blockIdx.x - tiles, gridDim.x - tiles);
     return;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) *spanCount = 0;
+  if (blockIdx.x == 0 && threadIdx.x < 2) spanCount[threadIdx.x] = 0;
   s_cnt[threadIdx.x] = 0;
   __syncthreads();
-  const u32 j0 = blockIdx.x * kLmSortTile + threadIdx.x;
+  const u32 j0 = blockIdx.x * (kLmThreads * R) + threadIdx.x;
+  u32 key[R];
 #pragma unroll
-  for (int r = 0; r < kLmSortRounds; ++r) {
+  for (int r = 0; r < R; ++r) {
     const u32 j = j0 + (u32)r * kLmThreads;
-    if (j < n) atomicAdd(&s_cnt[(keys(j).key >> shift) & mask], 1u);
+    key[r] = keys.key(j < n ? j : n - 1);
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (j0 + (u32)r * kLmThreads < n) atomicAdd(&s_cnt[(key[r] >> shift) & mask], 1u);
   __syncthreads();
-  counts[threadIdx.x * (u64)tiles + blockIdx.x] = s_cnt[threadIdx.x];
+  counts[tiles <= kLmSortOwn ? blockIdx.x * (u64)kLmBins + threadIdx.x : threadIdx.x * (u64)tiles + blockIdx.x] = s_cnt[threadIdx.x];
 }
 
-// ... per digit the exclusive sums over the tiles and the total, a wavefront a digit ...
+// ... per digit the exclusive sums over the tiles and the total, a workgroup a digit ...
+constexpr int kLmScanPer = 8;
 __global__ void __launch_bounds__(kLmThreads) k_lm_sort_scan(u32* __restrict__ counts, u32 tiles, u32* __restrict__ totals) {
-  const int lane = (int)(threadIdx.x & 63);
-  const u32 bin = blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6);
-  u32* c = counts + bin * (u64)tiles;
+  __shared__ u32 s_part[4];
+  const int lane = (int)(threadIdx.x & 63), wv = (int)(threadIdx.x >> 6);
+  u32* c = counts + blockIdx.x * (u64)tiles;
   u32 run = 0;
-  for (u32 i0 = 0; i0 < tiles; i0 += 64) {
-    const u32 i = i0 + (u32)lane;
-    const u32 x = i < tiles ? c[i] : 0u;
-    const u32 incl = lm_scan_incl(x, lane);
-    if (i < tiles) c[i] = run + incl - x;
-    run += wave_bcast_u32(incl, 63);
+  for (u32 i0 = 0; i0 < tiles; i0 += kLmThreads * kLmScanPer) {
+    u32 x[kLmScanPer], sum = 0;
+    const u32 i = i0 + threadIdx.x * kLmScanPer;
+#pragma unroll
+    for (int k = 0; k < kLmScanPer; ++k) x[k] = i + (u32)k < tiles ? c[i + (u32)k] : 0u;
+#pragma unroll
+    for (int k = 0; k < kLmScanPer; ++k) sum += x[k];
+    const u32 incl = lm_scan_incl(sum, lane);
+    if (lane == 63) s_part[wv] = incl;
+    __syncthreads();
+    u32 before = run + incl - sum;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wv) before += s_part[w];
+      run += s_part[w];
+    }
+#pragma unroll
+    for (int k = 0; k < kLmScanPer; ++k) {
+      if (i + (u32)k < tiles) c[i + (u32)k] = before;
+      before += x[k];
+    }
+    __syncthreads();
   }
-  if (lane == 0) totals[bin] = run;
+  if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
-// ... and every key to its place
-template <class Keys>
+// ... and every entry to its place
+template <int R, class E, class Keys>
 __global__ void __launch_bounds__(kLmThreads)
     k_lm_sort_scatter(Keys keys, u32 n, u32 shift, u32 bits, const u32* __restrict__ counts, u32 tiles, const u32* __restrict__ totals,
-                      LmPair* __restrict__ out) {
+                      E* __restrict__ out) {
   constexpr int kWaves = kLmThreads / 64;
   __shared__ u32 s_cnt[kWaves][kLmBins];
   __shared__ u32 s_bin[kLmBins];
   __shared__ u32 s_part[4];
   const int lane = (int)(threadIdx.x & 63), wv = (int)(threadIdx.x >> 6);
   const u32 mask = (1u << bits) - 1;
-  const u32 mine = counts[threadIdx.x * (u64)tiles + blockIdx.x];
-  s_bin[threadIdx.x] = totals[threadIdx.x];
+  const u32 pos0 = blockIdx.x * (kLmThreads * R) + (u32)wv * (64u * R) + (u32)lane;
+  E p[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const u32 j = pos0 + 64u * (u32)r;
+    p[r] = keys.entry(j < n ? j : n - 1);
+  }
+  // of this thread's digit: entries in earlier tiles, in all
+  u32 mine = 0, total = 0;
+  if (tiles <= kLmSortOwn) {
+#pragma unroll 16
+    for (u32 t = 0; t < tiles; ++t) {
+      const u32 x = counts[t * (u64)kLmBins + threadIdx.x];
+      mine += t < blockIdx.x ? x : 0u;
+      total += x;
+    }
+  } else {
+    mine = counts[threadIdx.x * (u64)tiles + blockIdx.x];
+    total = totals[threadIdx.x];
+  }
+  s_bin[threadIdx.x] = total;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) s_cnt[w][threadIdx.x] = 0;
-  const u32 pos0 = blockIdx.x * kLmSortTile + (u32)wv * (64u * kLmSortRounds) + (u32)lane;
-  LmPair p[kLmSortRounds];
-#pragma unroll
-  for (int r = 0; r < kLmSortRounds; ++r) {
-    p[r] = LmPair{0, 0};
-    if (pos0 + 64u * (u32)r < n) p[r] = keys(pos0 + 64u * (u32)r);
-  }
   __syncthreads();
   lm_scan_bins(s_bin, s_part, lane, wv);
-  u32 rank[kLmSortRounds];
+  u32 rank[R];
 #pragma unroll
-  for (int r = 0; r < kLmSortRounds; ++r)
+  for (int r = 0; r < R; ++r)
     rank[r] = lm_rank_round((p[r].key >> shift) & mask, pos0 + 64u * (u32)r < n, bits, s_cnt[wv], lane);
   __syncthreads();
   {
     u32 run = s_bin[threadIdx.x] + mine;
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const u32 x = s_cnt[w][threadIdx.x];
       s_cnt[w][threadIdx.x] = run;
@@ -300,21 +358,21 @@ __global__ void __launch_bounds__(kLmThreads)
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kLmSortRounds; ++r)
+  for (int r = 0; r < R; ++r)
     if (pos0 + 64u * (u32)r < n) out[s_cnt[wv][(p[r].key >> shift) & mask] + rank[r]] = p[r];
 }
 
 // ---- sums by word ----------------------------------------------------------------
+template <class E>
 struct LmSeg {
-  const LmPair* pairs;   // sorted
+  const E* entries;      // sorted
   u32 n;
-  u32 tile;              // entries of a tile, a multiple of 8, at most 64
+  u32 part;              // entries of a group, a multiple of 8
+  u32 tile;              // entries of a workgroup
   u32 tiles;
   u32 vocab, dim, colBlocks;
-  u32 perToken;          // entries of a row of src
-  float scale;           // weight of every entry ...
-  const float* weights;  // ... or of each
-  i64 srcStride;
+  float scale;           // weight of every entry that has none of its own
+  u32 srcStride;
   float* grad;
   i64 gradStride;
   float* head;           // [tiles][dim] partial row of the word that began in an earlier tile
@@ -323,77 +381,138 @@ struct LmSeg {
   u32* spanCount;
 };
 
-template <class T, int V>
-__global__ void __launch_bounds__(kLmThreads) k_lm_seg_sum(LmSeg q, const typename T::store* __restrict__ src) {
-  const int lane = (int)(threadIdx.x & 63);
-  const u64 tasks = (u64)q.tiles * q.colBlocks;
-  for (u64 task = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6); task < tasks; task += (u64)gridDim.x * (kLmThreads / 64)) {
-    const u32 tile = uni((u32)(task / q.colBlocks));
-    const u32 cb = uni((u32)(task - (u64)tile * q.colBlocks));
-    const u32 j0 = tile * q.tile;
-    const u32 cnt = uni(q.n - j0 < q.tile ? q.n - j0 : q.tile);
-    const bool on = (cb * 64u + (u32)lane) * V < q.dim;
-    const u32 col = on ? lm_col<V>(cb * 64u + (u32)lane, q.dim) : 0u;
-    LmPair p = {q.vocab, 0};
-    if ((u32)lane < cnt) p = q.pairs[j0 + (u32)lane];
-    const u32 prevKey = tile > 0 ? q.pairs[j0 - 1].key : ~0u;
-    const u32 nextKey = j0 + cnt < q.n ? q.pairs[j0 + cnt].key : ~0u;
-    float w = q.scale;
-    if (q.weights != nullptr) w = p.key < q.vocab ? q.weights[p.entry] : 0.f;
-    const u32 srow = q.perToken > 1 ? p.entry / q.perToken : p.entry;
-    u32 cur = wave_bcast_u32(p.key, 0);
-    bool first = cur == prevKey;   // the running word began in an earlier tile
+// A group of L lanes owns L V columns of `part` entries; a workgroup's groups, in order, own its tile.  The rows of src are
+// the bytes that count.  For the lookup's gradient each is read once and a group takes as much of it as it can (L V >= dim).
+// For the loss each is read by every candidate of its token, from anywhere in the chip: there a group takes one cache line
+// of a row, and as the workgroups of a tile's column blocks go round the XCDs, an XCD sees a part of src's columns only,
+// most of which its own L2 then holds (half lines, eight blocks of 256 columns of bf16, were no use: the L2 fetches whole
+// ones).
+template <class T, int V, int L, class E>
+__global__ void __launch_bounds__(kLmThreads) k_lm_seg_sum(LmSeg<E> q, const typename T::store* __restrict__ src) {
+  constexpr int kGroups = kLmThreads / L, kCols = L * V;
+  __shared__ float s_head[kGroups][kCols];
+  __shared__ float s_tail[kGroups][kCols];
+  __shared__ u32 s_flags[kGroups];      // 1: head, 2: the head's word goes on, 4: tail
+  __shared__ u32 s_headKey[kGroups];
+  const u32 gl = threadIdx.x & (L - 1), grp = threadIdx.x / L;
+  const u64 blocks = (u64)q.tiles * q.colBlocks;
+  for (u64 block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const u32 cb = (u32)(block % q.colBlocks), tile = (u32)(block / q.colBlocks);
+    const u32 pack = cb * L + gl;
+    const bool on = pack * V < q.dim;
+    const u32 col = on ? lm_col<V>(pack, q.dim) : 0u;
+    const u32 j0 = tile * q.tile + grp * q.part;
+    const u32 cnt = j0 < q.n ? (q.n - j0 < q.part ? q.n - j0 : q.part) : 0u;
     float acc[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.f;
-    auto put = [&](float* row) {
-      if (on) lm_store<LmF32, V>(row + col, lm_pack<LmF32, V>(acc));
-    };
-    for (u32 i0 = 0; i0 < cnt && cur < q.vocab; i0 += 8) {
-      LmPack<T, V> x[8];
-      // (entries that name no word are last and read row 0 of src's own rows: their entry is in range)
+    u32 flags = 0, headKey = 0;
+    if (cnt > 0) {
+      const u32 prevKey = j0 > 0 ? q.entries[j0 - 1].key : ~0u;
+      const u32 nextKey = j0 + cnt < q.n ? q.entries[j0 + cnt].key : ~0u;
+      u32 cur = q.entries[j0].key;
+      headKey = cur;
+      bool first = cur == prevKey;   // the running word began in an earlier part
+      auto load8 = [&](E (&p)[8], u32 i0) {
 #pragma unroll
-      for (u32 i = 0; i < 8; ++i) {
-        const u32 at = i0 + i < cnt ? i0 + i : cnt - 1;
-        const u32 r = wave_bcast_u32(srow, (int)at);
-        x[i] = lm_load<T, V>(src + (i64)r * q.srcStride + col);
-      }
+        for (u32 i = 0; i < 8; ++i) p[i] = q.entries[j0 + (i0 + i < cnt ? i0 + i : cnt - 1)];
+      };
+      E p[8];
+      load8(p, 0);
+      for (u32 i0 = 0; i0 < cnt && cur < q.vocab; i0 += 8) {
+        LmPack<T, V> x[8];
+        u32 key[8];
+        float w[8];
 #pragma unroll
-      for (u32 i = 0; i < 8; ++i) {
-        if (i0 + i < cnt) {
-          const u32 key = wave_bcast_u32(p.key, (int)(i0 + i));
-          const float wi = wave_bcast_f32(w, (int)(i0 + i));
-          if (key != cur) {
-            if (cur < q.vocab) put(first ? q.head + (u64)tile * q.dim : q.grad + (i64)cur * q.gradStride);
-            first = false;
-            cur = key;
+        for (u32 i = 0; i < 8; ++i) {
+          x[i] = lm_load<T, V>(src + (u64)p[i].row * q.srcStride + col);   // (an entry that names no word has a row too)
+          key[i] = p[i].key;
+          if constexpr (E::kWeighted) w[i] = p[i].weight;
+          else w[i] = q.scale;
+        }
+        load8(p, i0 + 8 < cnt ? i0 + 8 : i0);
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] = 0.f;
-          }
-          if (key < q.vocab) {
+        for (u32 i = 0; i < 8; ++i) {
+          if (i0 + i < cnt) {
+            if (key[i] != cur) {
+              if (cur < q.vocab) {
+                if (first) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] = __builtin_fmaf(wi, x[i].get(e), acc[e]);
+                  for (int e = 0; e < V; ++e) s_head[grp][gl * V + (u32)e] = acc[e];
+                  flags |= 1;
+                } else if (on) {
+                  lm_store<LmF32, V>(q.grad + (i64)cur * q.gradStride + col, lm_pack<LmF32, V>(acc));
+                }
+              }
+              first = false;
+              cur = key[i];
+#pragma unroll
+              for (int e = 0; e < V; ++e) acc[e] = 0.f;
+            }
+            if (cur < q.vocab) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) acc[e] = __builtin_fmaf(w[i], x[i].get(e), acc[e]);
+            }
           }
         }
       }
-    }
-    if (cur < q.vocab) {
-      if (first) {
-        put(q.head + (u64)tile * q.dim);
-      } else if (cur == nextKey) {
-        put(q.tail + (u64)tile * q.dim);
-        if (cb == 0 && lane == 0) q.span[atomicAdd(q.spanCount, 1u)] = tile;
-      } else {
-        put(q.grad + (i64)cur * q.gradStride);
+      if (cur < q.vocab) {
+        const bool on2 = cur == nextKey;   // goes on behind the part
+        if (first) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) s_head[grp][gl * V + (u32)e] = acc[e];
+          flags |= on2 ? 3 : 1;
+        } else if (on2) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) s_tail[grp][gl * V + (u32)e] = acc[e];
+          flags |= 4;
+        } else if (on) {
+          lm_store<LmF32, V>(q.grad + (i64)cur * q.gradStride + col, lm_pack<LmF32, V>(acc));
+        }
       }
     }
+    if (gl == 0) {
+      s_flags[grp] = flags;
+      s_headKey[grp] = headKey;
+    }
+    __syncthreads();
+    // the words that cross parts, a thread a column, the parts in order
+    for (u32 c = threadIdx.x; c < (u32)kCols; c += kLmThreads) {
+      const u32 pk = cb * L + c / V;
+      if (pk * V >= q.dim) continue;
+      const u32 cc = lm_col<V>(pk, q.dim) + c % V;
+      float run = 0.f;
+      bool outside = true, open = false;   // the word began in an earlier tile; it goes on
+      for (int g = 0; g < kGroups; ++g) {
+        const u32 f = s_flags[g];
+        if ((f & 1) != 0) {
+          run += s_head[g][c];
+          open = (f & 2) != 0;
+          if (!open) {
+            if (outside) q.head[(u64)tile * q.dim + cc] = run;
+            else q.grad[(i64)s_headKey[g] * q.gradStride + cc] = run;
+          }
+        }
+        if ((f & 4) != 0) {
+          run = s_tail[g][c];
+          outside = false;
+          open = true;
+        }
+      }
+      if (open) {
+        (outside ? q.head : q.tail)[(u64)tile * q.dim + cc] = run;
+        if (!outside && c == 0 && cb == 0) q.span[atomicAdd(q.spanCount, 1u)] = tile;
+      }
+    }
+    __syncthreads();   // (the next tile writes what this one reads)
   }
 }
 
 // A word over several tiles: tail of the first, heads of the following ones.  A workgroup takes 64 columns of a word; its
 // wavefronts take consecutive parts of the tiles, and their sums are added in that order.
-constexpr int kLmJoinWaves = 8;
-__global__ void __launch_bounds__(64 * kLmJoinWaves) k_lm_seg_join(LmSeg q) {
+constexpr int kLmJoinWaves = 4;
+template <class E>
+__global__ void __launch_bounds__(64 * kLmJoinWaves) k_lm_seg_join(LmSeg<E> q) {
   __shared__ float s_sum[kLmJoinWaves][64];
   const int lane = (int)(threadIdx.x & 63), wv = (int)(threadIdx.x >> 6);
   const u32 colBlocks = (q.dim + 63) / 64;
@@ -401,12 +520,12 @@ __global__ void __launch_bounds__(64 * kLmJoinWaves) k_lm_seg_join(LmSeg q) {
   for (u64 task = blockIdx.x; task < tasks; task += gridDim.x) {
     const u32 a = q.span[task / colBlocks];
     const u32 col = (u32)(task % colBlocks) * 64u + (u32)lane;
-    const u32 key = q.pairs[(a + 1) * q.tile - 1].key;
+    const u32 key = q.entries[(a + 1) * q.tile - 1].key;
     // tiles a + 1 .. b start with the word
     u32 b = a + 1;
     for (;;) {
       const u32 t = b + 1 + (u32)lane;
-      const u64 m = wave_ballot(t < q.tiles && q.pairs[(u64)t * q.tile].key == key);
+      const u64 m = wave_ballot(t < q.tiles && q.entries[(u64)t * q.tile].key == key);
       const u32 k = ~m == 0 ? 64u : (u32)__builtin_ctzll(~m);
       b += k;
       if (k < 64) break;

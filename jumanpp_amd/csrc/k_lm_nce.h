@@ -252,10 +252,10 @@ __global__ void __launch_bounds__(kLmThreads)
         rowL = (u32)lane < kn ? lm_row(ids, t * q.cands + kb + (u32)lane, q.vocab) : q.vocab;
         lnL = rowL < q.vocab ? q.logNoise[rowL] : 0.f;
       }
-      const float biasL = q.constant + lnL;
+      // (no word: a bias that nothing with one has)
+      const float biasL = rowL < q.vocab ? q.constant + lnL : __builtin_nanf("");
       // (a candidate that names no word reads the target's row and leaves with a gradient of zero)
       const u64 atL = (u64)(rowL < q.vocab ? rowL : target) * (u64)q.tableStride;
-      const u64 okL64 = wave_ballot(rowL < q.vocab);
       // lane k keeps what is candidate k's alone: its logit now, its loss and gradient once for all 64 behind the loop.  In
       // the loop a group makes the gradient of its candidate only as far as dh needs it.
       float zL = 0.f;
@@ -272,7 +272,6 @@ __global__ void __launch_bounds__(kLmThreads)
         for (int u = 0; u < U; ++u) {
           const u32 k = k0 + (u32)u * kGroups + grp;
           if (k0 + (u32)u * kGroups >= kn) continue;
-          const bool ok = k < kn && ((okL64 >> (k & 63)) & 1) != 0;
           float dot;
           if constexpr (BLOCKS) {
             dot = lm_dot_blocks<T, V, G, NV>(h + (i64)t * q.hStride, table + at[u], gl, shape);
@@ -281,7 +280,8 @@ __global__ void __launch_bounds__(kLmThreads)
             dot = hr.template dot<T, G>(b[u]);
           }
           dot = lm_group_sum<G>(dot);
-          const float z = dot - wave_shfl_f32(biasL, (int)(k & 63));
+          const float bias = wave_shfl_f32(biasL, (int)(k & 63));
+          const float z = dot - bias;
           // (lane k of the 64 reads group k mod kGroups)
           const float mine = kGroups == 1 ? z : wave_shfl_f32(z, (int)(((u32)lane & (kGroups - 1)) * G));
           const u32 k1 = k0 + (u32)u * kGroups;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kLmThreads)
           if (DH && !BLOCKS) {
             float a, c;
             lm_gate(kb + k == 0 ? -z : z, a, c);
-            if (ok) acc.template add<T, G>(kb + k == 0 ? -a * w : a * w, b[u]);
+            if (k < kn && bias == bias) acc.template add<T, G>(kb + k == 0 ? -a * w : a * w, b[u]);
           }
         }
       }
@@ -319,18 +319,39 @@ __global__ void __launch_bounds__(kLmThreads)
         }
       }
     } else {
-      // the groups' parts, in a fixed tree
+      if constexpr (DH && G == 64) {
+        acc.template store<T, G>(dh + (i64)t * q.dhStride, 0, gl, shape);
+      } else if constexpr (DH) {
+        // the four groups' parts are added and shared out: group r stores a quarter of every lane's elements
+        static_assert(G == 16, "a group is a row of lanes");
+        constexpr int Q = NV * V / 4;
+        float flat[NV * V];
 #pragma unroll
-      for (int d = G; d < 64; d *= 2) {
-        if (DH) {
+        for (int i = 0; i < NV * V; ++i) flat[i] = acc.p[i / V][i % V];
+        lm_rows_share(flat);
+        float mine[Q];
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < Q; ++i) mine[i] = flat[i];
+        typename T::store* row = dh + (i64)t * q.dhStride;
+        constexpr int kStore = Q < V ? Q : V;   // elements of one pack that a group has
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc.p[i][e] += wave_shfl_f32(acc.p[i][e], lane ^ d);
-          acc.tail += wave_shfl_f32(acc.tail, lane ^ d);
+        for (int i = 0; i < Q; i += kStore) {
+          const u32 at = grp * (u32)Q + (u32)i, pack = gl + G * (at / V);
+          float part[kStore];
+#pragma unroll
+          for (int e = 0; e < kStore; ++e) part[e] = mine[i + e];
+          if (FULL || pack < shape.packs) lm_store<T, kStore>(row + pack * V + at % V, lm_pack<T, kStore>(part));
+        }
+        if constexpr (!FULL) {
+          if (shape.rest != 0) {
+            float tail = acc.tail;
+            tail += wave_shfl_f32(tail, lane ^ 32);
+            tail += wave_shfl_f32(tail, lane ^ 16);
+            const float one[1] = {tail};
+            if (grp == 0 && gl < shape.rest) lm_store<T, 1>(row + shape.packs * V + gl, lm_pack<T, 1>(one));
+          }
         }
       }
-      if (DH && grp == 0) acc.template store<T, G>(dh + (i64)t * q.dhStride, 0, gl, shape);
     }
     loss = lm_group_sum<64>(loss);
     if (lane == 0) q.out[t] = live ? loss * w : 0.f;

@@ -15,8 +15,8 @@ rows and n + 1 int32 offsets, as jppgpu_analyze_batch takes its sentences.
 There is no CPU implementation behind this module.  (tests/ pass `lib_path` of the emulator build; test infrastructure.)
 """
 import ctypes as C
+import functools
 import struct
-import threading
 
 import torch
 
@@ -116,22 +116,20 @@ def _vector(t, what, n, dtype):
     return t.data_ptr()
 
 
-_need = threading.local()
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(lib, name, *sizes):
+    need = C.c_uint64()
+    _check(lib, getattr(lib, name)(*sizes, C.addressof(need)))
+    return need.value
 
 
-def _workspace(lib, fn, args, device):
+def _workspace(lib, name, sizes, like):
     """(tensor or None, pointer, bytes) of a workspace; torch's allocator keeps it for the stream, or for the graph"""
-    try:
-        need, at = _need.value
-    except AttributeError:
-        need = C.c_uint64()
-        at = C.addressof(need)
-        _need.value = need, at
-    _check(lib, fn(*args, at))
-    if need.value == 0:
+    need = _workspace_bytes(lib, name, *sizes)
+    if need == 0:
         return None, 0, 0
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-    return ws, ws.data_ptr(), need.value
+    ws = like.new_empty(need, dtype=torch.uint8)
+    return ws, ws.data_ptr(), need
 
 
 def embed(table, ids, scale=1.0, dtype=None, lib_path=None):
@@ -143,7 +141,7 @@ def embed(table, ids, scale=1.0, dtype=None, lib_path=None):
         _refuse('ids have %d dimensions, not 1' % ids.dim())
     rows, idv = _rows(table, 'table'), _ids(ids)
     n, (vocab, dim) = ids.shape[0], table.shape
-    out = torch.empty((n, dim), dtype=dtype or table.dtype, device=table.device)
+    out = table.new_empty((n, dim), dtype=dtype)
     _check(lib, lib.jppgpu_lm_embed(rows, vocab, dim, idv, n, scale, _out(out, dim), dev, stream))
     return out
 
@@ -156,8 +154,8 @@ def embed_grad(dy, ids, vocab, scale=1.0, lib_path=None):
         _refuse('ids are %s, dy has %d rows' % (tuple(ids.shape), dy.shape[0]))
     rows, idv = _rows(dy, 'dy'), _ids(ids)
     n, dim = dy.shape
-    ws, wp, wn = _workspace(lib, lib.jppgpu_lm_embed_grad_workspace, (n, vocab, dim), dy.device)
-    grad = torch.empty((vocab, dim), dtype=torch.float32, device=dy.device)
+    ws, wp, wn = _workspace(lib, 'jppgpu_lm_embed_grad_workspace', (n, vocab, dim), dy)
+    grad = dy.new_empty((vocab, dim), dtype=torch.float32)
     _check(lib, lib.jppgpu_lm_embed_grad(rows, idv, n, vocab, dim, scale, _out(grad, dim), wp, wn, dev, stream))
     return grad
 
@@ -185,10 +183,10 @@ def scan(gate, x, offsets=None, state=None, max_len=None, save=False, lib_path=N
     offsets, op, n = _batch(offsets, rows, x.device)
     sv = _rows(state, 'state', n, dim) if state is not None else None
     max_len = max_len or 0
-    h = torch.empty((rows, dim), dtype=x.dtype, device=x.device)
-    last = torch.empty((n, dim), dtype=torch.float32, device=x.device)
-    saved = torch.empty((lib.jppgpu_lm_scan_saved(rows), dim), dtype=torch.float32, device=x.device) if save else None
-    ws, wp, wn = _workspace(lib, lib.jppgpu_lm_scan_workspace, (rows, n, dim, max_len), x.device)
+    h = x.new_empty((rows, dim))
+    last = x.new_empty((n, dim), dtype=torch.float32)
+    saved = x.new_empty((lib.jppgpu_lm_scan_saved(rows), dim), dtype=torch.float32) if save else None
+    ws, wp, wn = _workspace(lib, 'jppgpu_lm_scan_workspace', (rows, n, dim, max_len), x)
     _check(lib, lib.jppgpu_lm_scan(gv, xv, op, n, rows, dim, max_len, sv, _out(h, dim), _out(last, dim),
                                    saved.data_ptr() if save else None, wp, wn, dev, stream))
     return (h, last, saved) if save else (h, last)
@@ -208,9 +206,9 @@ def scan_grad(gate, x, dh, saved, offsets=None, state=None, dlast=None, max_len=
     if saved.dtype != torch.float32 or tuple(saved.shape) != (lib.jppgpu_lm_scan_saved(rows), dim) or not saved.is_contiguous():
         _refuse('saved is not what scan(..., save=True) returned for these rows')
     max_len = max_len or 0
-    dgate, dx = (torch.empty((rows, dim), dtype=x.dtype, device=x.device) for _ in range(2))
-    dstate = torch.empty((n, dim), dtype=torch.float32, device=x.device)
-    ws, wp, wn = _workspace(lib, lib.jppgpu_lm_scan_workspace, (rows, n, dim, max_len), x.device)
+    dgate, dx = x.new_empty((rows, dim)), x.new_empty((rows, dim))
+    dstate = x.new_empty((n, dim), dtype=torch.float32)
+    ws, wp, wn = _workspace(lib, 'jppgpu_lm_scan_workspace', (rows, n, dim, max_len), x)
     _check(lib, lib.jppgpu_lm_scan_grad(gv, xv, op, n, rows, dim, max_len, sv, saved.data_ptr(), dv, lv, _out(dgate, dim),
                                         _out(dx, dim), _out(dstate, dim), wp, wn, dev, stream))
     return dgate, dx, dstate
@@ -229,7 +227,7 @@ def nce_score(h, table, ids, constant, lib_path=None):
     dev, stream = _where(lib_path, h, table, ids)
     hv, tv, idv = _rows(h, 'h'), _rows(table, 'table'), _ids(ids)
     _candidates(h, table, ids)
-    scores = torch.empty(tuple(ids.shape), dtype=torch.float32, device=h.device)
+    scores = h.new_empty(ids.shape, dtype=torch.float32)
     _check(lib, lib.jppgpu_lm_nce_score(hv, tv, table.shape[0], table.shape[1], idv, ids.shape[0], ids.shape[1], constant,
                                         scores.data_ptr(), dev, stream))
     return scores
@@ -248,14 +246,14 @@ def nce_loss(h, table, ids, log_noise, constant, weight=None, grads=True, lib_pa
     vocab, dim = table.shape
     ln = _vector(log_noise, 'log_noise', vocab, torch.float32)
     wt = _vector(weight, 'weight', n, torch.float32) if weight is not None else None
-    loss = torch.empty(n, dtype=torch.float32, device=h.device)
+    loss = h.new_empty(n, dtype=torch.float32)
     if not grads:
         _check(lib, lib.jppgpu_lm_nce_loss(hv, tv, vocab, dim, idv, n, cands, ln, constant, wt, loss.data_ptr(), None, None,
                                            None, 0, dev, stream))
         return loss
-    ws, wp, wn = _workspace(lib, lib.jppgpu_lm_nce_loss_workspace, (n, cands, vocab, dim), h.device)
-    dh = torch.empty((n, dim), dtype=h.dtype, device=h.device)
-    dtable = torch.empty((vocab, dim), dtype=torch.float32, device=h.device)
+    ws, wp, wn = _workspace(lib, 'jppgpu_lm_nce_loss_workspace', (n, cands, vocab, dim), h)
+    dh = h.new_empty((n, dim))
+    dtable = h.new_empty((vocab, dim), dtype=torch.float32)
     _check(lib, lib.jppgpu_lm_nce_loss(hv, tv, vocab, dim, idv, n, cands, ln, constant, wt, loss.data_ptr(), _out(dh, dim),
                                        _out(dtable, dim), wp, wn, dev, stream))
     return loss, dh, dtable

@@ -125,7 +125,7 @@ def raw_grad(E, dy, ids, vocab, scale, stride=None):
     lib = lm._lib(E.lib_path)
     n, dim = dy.shape
     grad = torch.full((vocab, stride or dim), float('nan'), device=E.device)
-    ws, wp, wn = lm._workspace(lib, lib.jppgpu_lm_embed_grad_workspace, (n, vocab, dim), dy.device)
+    ws, wp, wn = lm._workspace(lib, 'jppgpu_lm_embed_grad_workspace', (n, vocab, dim), dy)
     if ws is not None:
         ws.fill_(255)
     dev, stream = lm._where(E.lib_path, dy, ids)
@@ -188,7 +188,7 @@ def raw_scan(E, gate, x, offsets, state, max_len, fill):
     h = E.to(fill.to(x.dtype))
     last = torch.full((n, dim), float('nan'), device=E.device)
     saved = torch.full((lib.jppgpu_lm_scan_saved(rows), dim), float('nan'), device=E.device)
-    ws, wp, wn = lm._workspace(lib, lib.jppgpu_lm_scan_workspace, (rows, n, dim, max_len), x.device)
+    ws, wp, wn = lm._workspace(lib, 'jppgpu_lm_scan_workspace', (rows, n, dim, max_len), x)
     if ws is not None:
         ws.fill_(255)
     dev, stream = lm._where(E.lib_path, x)
@@ -204,7 +204,7 @@ def raw_scan_grad(E, gate, x, offsets, state, max_len, saved, dh, dlast, fill):
     n = offsets.shape[0] - 1
     dgate, dx = (E.to(fill.to(x.dtype).clone()) for _ in range(2))
     dstate = torch.full((n, dim), float('nan'), device=E.device)
-    ws, wp, wn = lm._workspace(lib, lib.jppgpu_lm_scan_workspace, (rows, n, dim, max_len), x.device)
+    ws, wp, wn = lm._workspace(lib, 'jppgpu_lm_scan_workspace', (rows, n, dim, max_len), x)
     if ws is not None:
         ws.fill_(255)
     dev, stream = lm._where(E.lib_path, x)
@@ -338,7 +338,7 @@ def scan_bad_offsets_stay_inside(E, offsets):
         (hb, h), (lb, last), (sb, saved), (gb, dgate), (xb, dx), (tb, dstate) = (
             guarded(r) for r in (rows, n, lib.jppgpu_lm_scan_saved(rows), rows, rows, n))
         saved.fill_(0.5)
-        ws, wp, wn = lm._workspace(lib, lib.jppgpu_lm_scan_workspace, (rows, n, dim, max_len), 'cpu')
+        ws, wp, wn = lm._workspace(lib, 'jppgpu_lm_scan_workspace', (rows, n, dim, max_len), x)
         M = lambda t: lm._rows(t, 't')  # noqa: E731
         lm._check(lib, lib.jppgpu_lm_scan(M(gate), M(x), off.data_ptr(), n, rows, dim, max_len, M(state), M(h), M(last), saved.data_ptr(),
                                           wp, wn, 0, None))
@@ -405,7 +405,7 @@ def nce_one_gradient_at_a_time(E):
     dev, stream = lm._where(E.lib_path, h)
     for pick in ('dh', 'dtable'):
         a, b, c = torch.empty_like(loss), torch.empty_like(dh), torch.empty_like(dtable)
-        ws, wp, wn = lm._workspace(lib, lib.jppgpu_lm_nce_loss_workspace, (20, 7, 30, 36), h.device)
+        ws, wp, wn = lm._workspace(lib, 'jppgpu_lm_nce_loss_workspace', (20, 7, 30, 36), h)
         lm._check(lib, lib.jppgpu_lm_nce_loss(lm._rows(h, 'h'), lm._rows(table, 't'), 30, 36, lm._ids(ids), 20, 7, log_noise.data_ptr(), 1.0,
                                               weight.data_ptr(), a.data_ptr(), lm._rows(b, 'dh') if pick == 'dh' else None,
                                               lm._rows(c, 'dt') if pick == 'dtable' else None, wp, wn, dev, stream))
