@@ -254,13 +254,15 @@ __device__ __forceinline__ void lm_rows_share(float (&v)[N]) {
   auto exchange = [&](float& a, float& b, auto half) {   // a: the sum over the pair in the lower lanes, b's in the upper
 #if defined(__HIP_DEVICE_COMPILE__)
     const u32 x = __builtin_bit_cast(u32, a), y = __builtin_bit_cast(u32, b);
+    u32 p, q;   // (words of their own: a bit cast of the result's second element takes the first)
     if constexpr (decltype(half)::value == 32) {
       const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
-      a = __builtin_bit_cast(float, r[0]) + __builtin_bit_cast(float, r[1]);
+      p = r[0], q = r[1];
     } else {
       const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
-      a = __builtin_bit_cast(float, r[0]) + __builtin_bit_cast(float, r[1]);
+      p = r[0], q = r[1];
     }
+    a = __builtin_bit_cast(float, p) + __builtin_bit_cast(float, q);
 #else
     constexpr int d = decltype(half)::value;
     const bool up = (lane_id() & d) != 0;
