@@ -367,9 +367,9 @@ void launch_scan(Launcher& go, const LmScan<T>& q) {
     else go(k_lm_scan_seq<T, V, false, STREAM>, blocks, kLmThreads, q);
     return;
   }
-  const u64 blocks = div_up((u64)q.chunks * q.colBlocks, waves);
-  go(k_lm_scan_agg<T, V>, blocks, kLmThreads, q);
-  go(k_lm_scan_carry<false>, div_up(q.dim, 64), 64u * kLmCarryWaves, q.aggA, q.aggB, q.chunks, q.dim);
+  const u64 blocks = div_up((u64)q.chunks * q.colBlocks, waves), groups = div_up(q.chunks, kLmGroup) * q.colBlocks;
+  go(k_lm_scan_agg<T, V>, groups, kLmThreads, q);
+  go(k_lm_scan_carry<false>, div_up(q.dim, kLmCarryCols), kLmCarryCols * kLmCarryRuns, q.groupA, q.groupB, (u32)div_up(q.chunks, kLmGroup), q.dim);
   if (q.saved != nullptr) go(k_lm_scan_chunk<T, V, true, STREAM>, blocks, kLmThreads, q);
   else go(k_lm_scan_chunk<T, V, false, STREAM>, blocks, kLmThreads, q);
 }
@@ -381,9 +381,9 @@ void launch_scan_grad(Launcher& go, const LmScan<T>& q) {
     go(k_lm_scan_grad_seq<T, V, STREAM>, div_up((u64)q.n * q.colBlocks, waves), kLmThreads, q);
     return;
   }
-  const u64 blocks = div_up((u64)q.chunks * q.colBlocks, waves);
-  go(k_lm_scan_grad_agg<T, V>, blocks, kLmThreads, q);
-  go(k_lm_scan_carry<true>, div_up(q.dim, 64), 64u * kLmCarryWaves, q.aggA, q.aggB, q.chunks, q.dim);
+  const u64 blocks = div_up((u64)q.chunks * q.colBlocks, waves), groups = div_up(q.chunks, kLmGroup) * q.colBlocks;
+  go(k_lm_scan_grad_agg<T, V>, groups, kLmThreads, q);
+  go(k_lm_scan_carry<true>, div_up(q.dim, kLmCarryCols), kLmCarryCols * kLmCarryRuns, q.groupA, q.groupB, (u32)div_up(q.chunks, kLmGroup), q.dim);
   go(k_lm_scan_grad_chunk<T, V, STREAM>, blocks, kLmThreads, q);
 }
 
@@ -397,6 +397,13 @@ void launch_scan_any(Launcher& go, const LmScan<T>& q, bool grad) {
     if (stream) launch_scan_grad<T, V, true>(go, q);
     else launch_scan_grad<T, V, false>(go, q);
   }
+}
+
+void carve_maps(Carver& c, u64 chunks, u64 dim, float** aggA, float** aggB, float** groupA, float** groupB) {
+  *aggA = c.take<float>(chunks * dim);
+  *aggB = c.take<float>(chunks * dim);
+  *groupA = c.take<float>(div_up(chunks, kLmGroup) * dim);
+  *groupB = c.take<float>(div_up(chunks, kLmGroup) * dim);
 }
 
 struct ScanArgs {
@@ -453,8 +460,7 @@ void run_scan(Launcher& go, const ScanArgs& s, bool grad) {
   if (q.chunk != 0) {
     q.chunks = (u32)div_up(q.rows, q.chunk);
     Carver c{static_cast<char*>(s.workspace)};
-    q.aggA = c.take<float>((u64)q.chunks * q.dim);
-    q.aggB = c.take<float>((u64)q.chunks * q.dim);
+    carve_maps(c, q.chunks, q.dim, &q.aggA, &q.aggB, &q.groupA, &q.groupB);
   }
   if (v == 1) launch_scan_any<T, 1>(go, q, grad);
   else if (v == 2) launch_scan_any<T, 2>(go, q, grad);
@@ -480,8 +486,8 @@ uint64_t scan_workspace(int64_t rows, int64_t n, int64_t dim, int64_t max_len) {
   const u32 chunk = scan_chunk((u64)rows, (u64)n, (u64)dim, (u64)max_len);
   if (chunk == 0) return 0;
   Carver c{nullptr};
-  c.take<float>(div_up((u64)rows, chunk) * (u64)dim);
-  c.take<float>(div_up((u64)rows, chunk) * (u64)dim);
+  float* none;
+  carve_maps(c, div_up((u64)rows, chunk), (u64)dim, &none, &none, &none, &none);
   return c.used;
 }
 

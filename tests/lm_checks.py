@@ -322,6 +322,7 @@ def scan_step_by_step_is_scan(E, long):
 def scan_bad_offsets_stay_inside(E, offsets):
     """offsets that fall or leave the batch: any values, but only in the outputs' own rows (the emulator's heap is checked by
     guard rows around every output)"""
+    assert not E.gpu, 'host memory: for the emulator alone'
     rows, dim = (700 if max(offsets) > 200 and max(offsets) < 2000 else 41), 10
     g = rng(1)
     gate, x, dh, state = normal(g, rows, dim), normal(g, rows, dim), normal(g, rows, dim), normal(g, len(offsets) - 1, dim)

@@ -2,7 +2,9 @@
 
 Every function returns (value, bound) pairs of float64 tensors.  A bound follows the operator's own recurrences with
 magnitudes in place of values; U is the largest relative rounding of a 32-bit operation.  What is counted:
-  a gate and its complement: exp within 3 U (reduction, table, product), 1 + e, the reciprocal, a product: 6 U
+  a gate and its complement: exp within 3 U (reduction, table, product), 1 + e, the reciprocal, a product: 6 U; for 16-bit
+  rows exp2(fl(-|z| fl(log2 e))): the product is off by U, the constant by 0.23 U of itself, which moves the power by 1.23
+  U |z|, on top of the exponential's 2 U, 1 + e, a reciprocal within 2 U and a product: (6 + 1.3 |z|) U
   a product or a sum: U each; a sum of n terms in any order: n U of the sum of magnitudes
 and the output's own rounding, half a unit of its type, on top.  Terms of order U^2 are covered by the slack factor 1.01.
 Every rule also allows the smallest numbers of the types to be flushed (TINY)."""
@@ -49,13 +51,15 @@ def embed_grad(dy, ids, vocab, scale):
 
 
 def _gates(gate):
+    """a, 1 - a and the relative rounding of either (beyond |z| = 104 both are 0 or 1)"""
     z = gate.double()
-    return torch.sigmoid(z), torch.sigmoid(-z)
+    err = torch.full_like(z, GATE) if gate.dtype == torch.float32 else (6 + 1.3 * z.abs().clamp(max=104)) * U
+    return torch.sigmoid(z), torch.sigmoid(-z), torch.nan_to_num(err)
 
 
 def scan(gate, x, offsets, state, dtype, fill):
     """h (rows of no sentence: `fill`), last"""
-    a, b = _gates(gate)
+    a, b, err = _gates(gate)
     xd = x.double()
     n, dim = len(offsets) - 1, x.shape[1]
     h = fill.double().clone()
@@ -70,7 +74,7 @@ def scan(gate, x, offsets, state, dtype, fill):
             v = a[t] * v + b[t] * xd[t]
             m = a[t] * m + b[t] * xd[t].abs()
             # the gates, the products and the sum of this row; in chunks the products of gates are rounded once more
-            e = a[t] * e + (GATE + 4 * U) * m
+            e = a[t] * e + (err[t] + 4 * U) * m
             h[t], hb[t] = v, e
         last[i], last_b[i] = v, e
     return out_round(h, hb, dtype), out_round(last, last_b, torch.float32), (before, before_b, before_m)
@@ -79,7 +83,7 @@ def scan(gate, x, offsets, state, dtype, fill):
 def scan_grad(gate, x, offsets, state, dh, dlast, dtype, fill):
     """dgate, dx (rows of no sentence: `fill`), dstate"""
     _, _, (before, before_b, before_m) = scan(gate, x, offsets, state, torch.float32, fill)
-    a, b = _gates(gate)
+    a, b, err = _gates(gate)
     xd, dhd = x.double(), dh.double()
     n, dim = len(offsets) - 1, x.shape[1]
     dgate, dx = fill.double().clone(), fill.double().clone()
@@ -91,11 +95,11 @@ def scan_grad(gate, x, offsets, state, dh, dlast, dtype, fill):
         for t in reversed(range(int(offsets[i]), int(offsets[i + 1]))):
             v, m = dhd[t] + v, dhd[t].abs() + m
             e = e + 2 * U * m
-            dx[t], dx_b[t] = v * b[t], b[t] * (e + (GATE + U) * m)
+            dx[t], dx_b[t] = v * b[t], b[t] * (e + (err[t] + U) * m)
             ab, diff, span = a[t] * b[t], before[t] - xd[t], before_m[t] + xd[t].abs()
             dgate[t] = v * ab * diff
-            dgate_b[t] = ab * (e * diff.abs() + m * before_b[t] + (2 * GATE + 5 * U) * m * span)
-            v, m, e = v * a[t], m * a[t], a[t] * (e + (GATE + 3 * U) * m)
+            dgate_b[t] = ab * (e * diff.abs() + m * before_b[t] + (2 * err[t] + 5 * U) * m * span)
+            v, m, e = v * a[t], m * a[t], a[t] * (e + (err[t] + 3 * U) * m)
         ds[i], ds_b[i] = v, e
     return out_round(dgate, dgate_b, dtype), out_round(dx, dx_b, dtype), out_round(ds, ds_b, torch.float32)
 
