@@ -3,6 +3,7 @@
 #define JPP_LM_H
 
 #include <cmath>
+#include <type_traits>
 
 #include "jpp_rt.h"
 
@@ -70,6 +71,22 @@ struct LmF16 {
 #endif
   }
 };
+
+// d + the products of two pairs of 16-bit elements, without taking them apart
+template <class T>
+__device__ __forceinline__ float lm_dot2(u32 a, u32 b, float d) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (std::is_same<T, LmBf16>::value) {
+    typedef __bf16 h2_t __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(h2_t, a), __builtin_bit_cast(h2_t, b), d, false);
+  } else {
+    typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, a), __builtin_bit_cast(h2_t, b), d, false);
+  }
+#else
+  return __builtin_fmaf(T::get(a >> 16), T::get(b >> 16), __builtin_fmaf(T::get(a & 0xffffu), T::get(b & 0xffffu), d));
+#endif
+}
 
 // N elements of a row, moved as one access of up to 16 bytes and held as the words that came.  (Held as an array of 16-bit
 // elements, a pack that is loaded under a condition is taken apart inside the branch, behind a wait of its own.)  The access

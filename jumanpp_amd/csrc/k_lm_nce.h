@@ -65,6 +65,23 @@ struct LmRowPart {
     }
   }
 };
+// the product of two parts; both cleared where they do not exist
+template <class T, int V, int G, int NV, bool FULL>
+__device__ __forceinline__ float lm_dot_parts(const LmRowPart<T, V, G, NV, FULL>& x, const LmRowPart<T, V, G, NV, FULL>& y) {
+  float d = 0.f;
+  if constexpr (!FULL) d = x.tail.get(0) * y.tail.get(0);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if constexpr (sizeof(typename T::store) == 2) {
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) d = lm_dot2<T>(x.p[i].w[k], y.p[i].w[k], d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d = __builtin_fmaf(x.p[i].get(e), y.p[i].get(e), d);
+    }
+  }
+  return d;
+}
 template <int V, int NV, bool FULL>
 struct LmRowSum {    // the same part in 32 bits
   float p[NV][V];
@@ -83,16 +100,6 @@ struct LmRowSum {    // the same part in 32 bits
 #pragma unroll
       for (int e = 0; e < V; ++e) p[i][e] = __builtin_fmaf(w, x.p[i].get(e), p[i][e]);
     if constexpr (!FULL) tail = __builtin_fmaf(w, x.tail.get(0), tail);
-  }
-  template <class T, int G>
-  __device__ __forceinline__ float dot(const LmRowPart<T, V, G, NV, FULL>& x) const {
-    float d = 0.f;
-    if constexpr (!FULL) d = tail * x.tail.get(0);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) d = __builtin_fmaf(p[i][e], x.p[i].get(e), d);
-    return d;
   }
   template <class T, int G>
   __device__ __forceinline__ void store(typename T::store* row, u32 p0, u32 gl, const LmRowShape& s) const {
@@ -118,10 +125,7 @@ __device__ __forceinline__ float lm_dot_blocks(const typename T::store* x, const
     b.load(y, p0, gl, s);
     a.mask(p0, gl, s);
     b.mask(p0, gl, s);
-    LmRowSum<V, NV, false> f;
-    f.zero();
-    f.template add<T, G>(1.f, a);
-    d += f.template dot<T, G>(b);
+    d += lm_dot_parts<T, V, G, NV, false>(a, b);
   }
   return d;
 }
@@ -160,13 +164,10 @@ __global__ void __launch_bounds__(kLmThreads)
     const u32 rowL = gl < cnt ? lm_row(ids, t * q.cands + k0 + gl, q.vocab) : q.vocab;
     float mine = 0.f;
     if (q.vocab != 0) {
-      LmRowSum<V, NV, FULL> hr;
+      LmRowPart<T, V, G, NV, FULL> hr;
       if constexpr (!BLOCKS) {
-        LmRowPart<T, V, G, NV, FULL> a;
-        a.load(h + (i64)t * q.hStride, 0, gl, shape);
-        a.mask(0, gl, shape);
-        hr.zero();
-        hr.template add<T, G>(1.f, a);
+        hr.load(h + (i64)t * q.hStride, 0, gl, shape);
+        hr.mask(0, gl, shape);
       }
       // (an id that names no word reads row 0 for nothing)
       const u64 atL = rowL < q.vocab ? (u64)rowL * (u64)q.tableStride : 0u;
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(kLmThreads)
               dot = lm_dot_blocks<T, V, G, NV>(h + (i64)t * q.hStride, table + at[u], gl, shape);
             } else {
               b[u].mask(0, gl, shape);
-              dot = hr.template dot<T, G>(b[u]);
+              dot = lm_dot_parts<T, V, G, NV, FULL>(hr, b[u]);
             }
             dot = lm_group_sum<G>(dot);
             if (gl == k + (u32)u) mine = dot;
@@ -236,14 +237,11 @@ __global__ void __launch_bounds__(kLmThreads)
     const u32 target = wave_bcast_u32(rowL, 0);
     const bool live = target < q.vocab;
     const float w = q.weight != nullptr ? q.weight[t] : 1.f;
-    LmRowSum<V, NV, FULL> hr, acc;
-    hr.zero();
+    LmRowSum<V, NV, FULL> acc;
     acc.zero();
     float loss = 0.f;
-    if constexpr (!BLOCKS) {
-      hN.mask(0, gl, shape);
-      hr.template add<T, G>(1.f, hN);
-    }
+    LmRowPart<T, V, G, NV, FULL> hr = hN;
+    if constexpr (!BLOCKS) hr.mask(0, gl, shape);
     fetch_ids(t + step);
     if (!live) fetch_rest(t + step);
     for (u32 kb = 0; live && kb < q.cands; kb += 64) {
@@ -277,7 +275,7 @@ __global__ void __launch_bounds__(kLmThreads)
             dot = lm_dot_blocks<T, V, G, NV>(h + (i64)t * q.hStride, table + at[u], gl, shape);
           } else {
             b[u].mask(0, gl, shape);
-            dot = hr.template dot<T, G>(b[u]);
+            dot = lm_dot_parts<T, V, G, NV, FULL>(hr, b[u]);
           }
           dot = lm_group_sum<G>(dot);
           const float bias = wave_shfl_f32(biasL, (int)(k & 63));

@@ -425,6 +425,35 @@ def nce_far_scores(E, z):
         near(name, a, b)
 
 
+@check(dtype=[BF16, F16], dim=[8, 40, 300])
+def nce_score_subnormal_rows(E, dim, dtype):
+    """the smallest numbers of a 16-bit table count in full: products of theirs with large states"""
+    g = rng(dim)
+    small = torch.finfo(dtype).smallest_normal
+    step = small * torch.finfo(dtype).eps
+    table = (torch.randint(-120, 121, (6, dim), generator=g).double() * step).to(dtype)
+    assert ((table.double().abs() < small) & (table != 0)).any()
+    h = normal(g, 5, dim, dtype=torch.float64, std=100.0 if dtype == F16 else 2.0 ** 110).to(dtype)
+    ids = words(g, 6, 5, 7, none=False)
+    near('score', lm.nce_score(E.to(h), E.to(table), E.to(ids), 0.0, **E.kw), R.nce_score(h, table, ids, 0.0)[:2])
+
+
+@check(dtype=[F32, BF16, F16])
+def nce_score_not_finite(E, dtype):
+    """an infinity or a NaN of a row is in the scores of that row and of no other"""
+    inf, nan = float('inf'), float('nan')
+    h = torch.ones(2, 32)
+    h[1, 5] = 0
+    table = torch.ones(5, 32)
+    table[1, 5], table[2, 6], table[3, 7], table[3, 8] = inf, -inf, inf, -inf
+    table[4, 31] = nan
+    ids = torch.tensor([[0, 1, 2, 3, 4, 9], [4, 3, 2, 1, 0, -1]], dtype=torch.int32)
+    got = lm.nce_score(E.to(h.to(dtype)), E.to(table.to(dtype)), E.to(ids), 2.0, **E.kw).cpu()
+    want = torch.tensor([[30, inf, -inf, nan, nan, -inf], [nan, nan, -inf, nan, 29, -inf]])
+    assert torch.equal(got.isnan(), want.isnan()), got
+    equal('scores', got[~got.isnan()], want[~want.isnan()])
+
+
 # ---- together --------------------------------------------------------------------------------------
 def chain_inputs(lengths, vocab, dim, k, seed, ids=None):
     """a model and a batch of sentences of word ids, as they come out of an analysis"""
