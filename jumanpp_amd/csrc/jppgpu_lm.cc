@@ -303,8 +303,10 @@ void sum_entries(Launcher& go, SumPlan& p, const SumSource& x) {
     default: launch_seg_sum<LmF16, E>(go, q, p.pack, p.lanes, x.src->data); break;
   }
   if (p.tiles > 1) {
-    const u64 most = (u64)p.tiles * div_up(p.dim, 64);
-    go(k_lm_seg_join<E>, most < 2048 ? most : 2048, 64u * kLmJoinWaves, q);
+    const u32 pack = p.dim < 4 ? 1 : 4;
+    const u64 most = (u64)p.tiles * div_up(p.dim, 64 * pack), blocks = most < 2048 ? most : 2048;
+    if (pack == 4) go(k_lm_seg_join<4, E>, blocks, 64u * kLmJoinWaves, q);
+    else go(k_lm_seg_join<1, E>, blocks, 64u * kLmJoinWaves, q);
   }
 }
 

@@ -508,18 +508,20 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_seg_sum(LmSeg<E> q, const typ
   }
 }
 
-// A word over several tiles: tail of the first, heads of the following ones.  A workgroup takes 64 columns of a word; its
+// A word over several tiles: tail of the first, heads of the following ones.  A workgroup takes 64 V columns of a word; its
 // wavefronts take consecutive parts of the tiles, and their sums are added in that order.
 constexpr int kLmJoinWaves = 4;
-template <class E>
+template <int V, class E>
 __global__ void __launch_bounds__(64 * kLmJoinWaves) k_lm_seg_join(LmSeg<E> q) {
-  __shared__ float s_sum[kLmJoinWaves][64];
+  constexpr u32 R = 8;   // partial rows in flight
+  __shared__ float s_sum[kLmJoinWaves][64 * V];
   const int lane = (int)(threadIdx.x & 63), wv = (int)(threadIdx.x >> 6);
-  const u32 colBlocks = (q.dim + 63) / 64;
+  const u32 packs = (q.dim + V - 1) / V, colBlocks = (packs + 63) / 64;
   const u64 tasks = (u64)*q.spanCount * colBlocks;
   for (u64 task = blockIdx.x; task < tasks; task += gridDim.x) {
     const u32 a = q.span[task / colBlocks];
-    const u32 col = (u32)(task % colBlocks) * 64u + (u32)lane;
+    const u32 pack = (u32)(task % colBlocks) * 64u + (u32)lane;
+    const u32 col = lm_col<V>(pack < packs ? pack : packs - 1, q.dim);
     const u32 key = q.entries[(a + 1) * q.tile - 1].key;
     // tiles a + 1 .. b start with the word
     u32 b = a + 1;
@@ -533,17 +535,29 @@ __global__ void __launch_bounds__(64 * kLmJoinWaves) k_lm_seg_join(LmSeg<E> q) {
     const u32 heads = b - a;
     const u32 per = (heads + kLmJoinWaves - 1) / kLmJoinWaves;
     const u32 h0 = a + 1 + per * (u32)wv, h1 = h0 + per < b + 1 ? h0 + per : b + 1;
-    float sum = 0.f;
-    if (col < q.dim) {
-      if (wv == 0) sum = q.tail[(u64)a * q.dim + col];
-#pragma unroll 8
-      for (u32 t = h0; t < h1; ++t) sum += q.head[(u64)t * q.dim + col];
+    LmPack<LmF32, V> x;
+    x.zero();
+    if (wv == 0) x = lm_load<LmF32, V>(q.tail + (u64)a * q.dim + col);
+    float sum[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[e] = x.get(e);
+    for (u32 t = h0; t < h1; t += R) {
+      LmPack<LmF32, V> y[R];
+#pragma unroll
+      for (u32 i = 0; i < R; ++i) y[i] = lm_load<LmF32, V>(q.head + (u64)(t + i < h1 ? t + i : t) * q.dim + col);
+#pragma unroll
+      for (u32 i = 0; i < R; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] += t + i < h1 ? y[i].get(e) : 0.f;
     }
-    s_sum[wv][lane] = sum;
+#pragma unroll
+    for (int e = 0; e < V; ++e) s_sum[wv][lane * V + e] = sum[e];
     __syncthreads();
-    if (wv == 0 && col < q.dim) {
-      for (int w = 1; w < kLmJoinWaves; ++w) sum += s_sum[w][lane];
-      q.grad[(i64)key * q.gradStride + col] = sum;
+    if (wv == 0) {
+      for (int w = 1; w < kLmJoinWaves; ++w)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] += s_sum[w][lane * V + e];
+      if (pack < packs) lm_store<LmF32, V>(q.grad + (i64)key * q.gradStride + col, lm_pack<LmF32, V>(sum));
     }
     __syncthreads();
   }
