@@ -98,7 +98,7 @@ int jppgpu_lm_nce_score(const jppgpu_lm_matrix* h, const jppgpu_lm_matrix* table
  * dh = d(sum of loss)/dh (n x dim, the type of h), dtable = d(sum of loss)/dtable (vocab x dim, 32-bit, written whole, summed
  * like jppgpu_lm_embed_grad).  A token without a following word (ids[t * cands] names none) has loss zero and no gradient,
  * whatever its row of h holds; a noise id that names no word is left out of the sum.  dh and dtable may have NULL data, both
- * or either: not wanted.  n * cands < 2^31.  The workspace is used where dtable is wanted. */
+ * or either: not wanted.  n * cands < 2^31.  The workspace is needed where either is wanted. */
 int jppgpu_lm_nce_loss_workspace(int64_t n, int64_t cands, int64_t vocab, int64_t dim, uint64_t* bytes);
 int jppgpu_lm_nce_loss(const jppgpu_lm_matrix* h, const jppgpu_lm_matrix* table, int64_t vocab, int64_t dim,
                        const jppgpu_lm_ids* ids, int64_t n, int64_t cands, const float* log_noise, float constant,

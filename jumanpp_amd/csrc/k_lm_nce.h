@@ -250,8 +250,8 @@ __global__ void __launch_bounds__(kLmThreads)
         rowL = (u32)lane < kn ? lm_row(ids, t * q.cands + kb + (u32)lane, q.vocab) : q.vocab;
         lnL = rowL < q.vocab ? q.logNoise[rowL] : 0.f;
       }
-      // (no word: a bias that nothing with one has)
-      const float biasL = rowL < q.vocab ? q.constant + lnL : __builtin_nanf("");
+      const u64 named = wave_ballot(rowL < q.vocab);
+      const float biasL = q.constant + lnL;
       // (a candidate that names no word reads the target's row and leaves with a gradient of zero)
       const u64 atL = (u64)(rowL < q.vocab ? rowL : target) * (u64)q.tableStride;
       // lane k keeps what is candidate k's alone: its logit now, its loss and gradient once for all 64 behind the loop.  In
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kLmThreads)
           if (DH && !BLOCKS) {
             float a, c;
             lm_gate(kb + k == 0 ? -z : z, a, c);
-            if (k < kn && bias == bias) acc.template add<T, G>(kb + k == 0 ? -a * w : a * w, b[u]);
+            if (((named >> (k & 63)) & 1u) != 0) acc.template add<T, G>(kb + k == 0 ? -a * w : a * w, b[u]);
           }
         }
       }

@@ -141,6 +141,8 @@ def embed(table, ids, scale=1.0, dtype=None, lib_path=None):
         _refuse('ids have %d dimensions, not 1' % ids.dim())
     rows, idv = _rows(table, 'table'), _ids(ids)
     n, (vocab, dim) = ids.shape[0], table.shape
+    if dtype is not None and dtype not in _TYPES:
+        _refuse('rows of %s; float32, bfloat16 and float16 are supported' % dtype)
     out = table.new_empty((n, dim), dtype=dtype)
     _check(lib, lib.jppgpu_lm_embed(rows, vocab, dim, idv, n, scale, _out(out, dim), dev, stream))
     return out
@@ -150,10 +152,10 @@ def embed_grad(dy, ids, vocab, scale=1.0, lib_path=None):
     """The gradient of embed's table, float32 [vocab, dim], from that of its result: rows summed by word in a fixed order."""
     lib = _lib(lib_path)
     dev, stream = _where(lib_path, dy, ids)
-    if ids.dim() != 1 or ids.shape[0] != dy.shape[0]:
-        _refuse('ids are %s, dy has %d rows' % (tuple(ids.shape), dy.shape[0]))
     rows, idv = _rows(dy, 'dy'), _ids(ids)
     n, dim = dy.shape
+    if ids.dim() != 1 or ids.shape[0] != n:
+        _refuse('ids are %s, dy has %d rows' % (tuple(ids.shape), n))
     ws, wp, wn = _workspace(lib, 'jppgpu_lm_embed_grad_workspace', (n, vocab, dim), dy)
     grad = dy.new_empty((vocab, dim), dtype=torch.float32)
     _check(lib, lib.jppgpu_lm_embed_grad(rows, idv, n, vocab, dim, scale, _out(grad, dim), wp, wn, dev, stream))

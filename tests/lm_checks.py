@@ -454,6 +454,32 @@ def nce_score_not_finite(E, dtype):
     equal('scores', got[~got.isnan()], want[~want.isnan()])
 
 
+@check(dtype=[F32, BF16], dim=[4, 1500])
+def nce_noise_without_a_logarithm(E, dim, dtype):
+    """noise probabilities of zero and infinity are probabilities; a NaN stays with the tokens whose candidate has it"""
+    inf, nan = float('inf'), float('nan')
+    h = torch.zeros(6, dim, dtype=torch.float64)
+    h[:, :4] = torch.tensor([1.0, 0.5, -1.0, 0.25])
+    table = torch.zeros(5, dim, dtype=torch.float64)
+    table[:, :4] = torch.arange(20).double().reshape(5, 4) / 16 - 0.5
+    ln = torch.tensor([-inf, inf, -1.0, nan, 0.5])
+    ids = torch.tensor([[0, 1, 4], [1, 2, 4], [2, 0, 4], [3, 2, 4], [2, 3, 2], [2, 4, 4]], dtype=torch.int32)
+    got = lm.nce_loss(E.to(h.to(dtype)), E.to(table.to(dtype)), E.to(ids), E.to(ln), 0.5, **E.kw)
+    sign = torch.tensor([-1.0, 1.0, 1.0], dtype=torch.float64)
+    rows = table[ids.long()]
+    z = (rows * h[:, None]).sum(-1) - 0.5 - ln.double()[ids.long()]
+    g = sign * torch.sigmoid(sign * z)
+    soft = torch.where((sign * z).isnan(), nan, torch.nn.functional.softplus(sign * z, threshold=1e9))
+    dtable = torch.zeros_like(table).index_add_(0, ids.long().reshape(-1), (g[:, :, None] * h[:, None]).reshape(-1, dim))
+    half = torch.finfo(dtype).eps / 2
+    # all terms are at most 4 in magnitude: z within 7 roundings of theirs, a sigmoid or softplus within 10, sums of at most 11
+    for what, a, want, out in zip(('loss', 'dh', 'dtable'), got, (soft.sum(1), (g[:, :, None] * rows).sum(1), dtable), (R.U, half, R.U)):
+        a = a.cpu().double()
+        assert torch.equal(a.isnan(), want.isnan()) and torch.equal(a.isinf(), want.isinf()), (what, a, want)
+        fine = want.isfinite()
+        assert ((a - want).abs()[fine] <= 4 * 28 * R.U + out * want.abs()[fine]).all(), (what, a, want)
+
+
 # ---- together --------------------------------------------------------------------------------------
 def chain_inputs(lengths, vocab, dim, k, seed, ids=None):
     """a model and a batch of sentences of word ids, as they come out of an analysis"""
@@ -564,6 +590,7 @@ def refusals(E):
         (lm.scan, (f(4, 8), f(4, 8), off), {'max_len': -1}), (lm.scan, (f(4, 8), f(4, 8), off[:0]), {}), (lm.scan, (f(4, 0), f(4, 0), off), {}),
         (lm.scan_grad, (f(4, 8), f(4, 8), f(4, 8, dtype=BF16), saved, off), {}), (lm.scan_grad, (f(4, 8), f(4, 8), f(4, 8), f(2, 8), off), {}),
         (lm.scan_grad, (f(4, 8), f(4, 8), f(3, 8), saved, off), {}), (lm.scan_grad, (f(4, 8), f(4, 8), f(4, 8), saved, off, None, f(1, 8)), {}),
+        (lm.embed, (f(5, 8), i(4)), {'dtype': torch.int32}), (lm.embed_grad, (f(8), i(8), 5), {}),
         (lm.nce_score, (f(4, 8), f(5, 9), i(4, 2), 0.0), {}), (lm.nce_score, (f(4, 8), f(5, 8), i(3, 2), 0.0), {}),
         (lm.nce_score, (f(4, 8), f(5, 8), i(4, 0), 0.0), {}), (lm.nce_score, (f(4, 8), f(5, 8, dtype=F16), i(4, 2), 0.0), {}),
         (lm.nce_loss, (f(4, 8), f(5, 8), i(4, 2), f(4), 0.0), {}), (lm.nce_loss, (f(4, 8), f(5, 8), i(4, 2), f(5, dtype=F16), 0.0), {}),
