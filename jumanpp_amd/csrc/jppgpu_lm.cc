@@ -356,8 +356,8 @@ u32 scan_chunk(u64 rows, u64 n, u64 dim, u64 maxLen) {
   const u64 blocks = div_up(dim, 256);
   if (longest <= 256) return 0;
   if (n * blocks >= 2048 && longest <= 4 * (rows / n)) return 0;
-  u64 chunk = div_up(div_up(rows * blocks, 4096), kLmSave) * kLmSave;
-  return (u32)(chunk < 32 ? 32 : chunk);
+  const u64 chunk = div_up(div_up(rows * blocks, 4096), kLmSave) * kLmSave;
+  return (u32)(chunk < 32 ? 32 : chunk < (1u << 30) ? chunk : 1u << 30);
 }
 
 template <class T, int V, bool STREAM>
