@@ -55,6 +55,14 @@ struct LmRowPart {
       if (s.rest != 0) tail = lm_load<T, 1>(row + s.packs * V + (gl < s.rest ? gl : 0u));
     }
   }
+  // cleared unless `ok`
+  __device__ __forceinline__ void keep(bool ok) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < LmPack<T, V>::kWords; ++k) p[i].w[k] = ok ? p[i].w[k] : 0u;
+    tail.w[0] = ok ? tail.w[0] : 0u;
+  }
   __device__ __forceinline__ void mask(u32 p0, u32 gl, const LmRowShape& s) {
     if constexpr (!FULL) {
 #pragma unroll
@@ -139,6 +147,12 @@ constexpr int lm_rows_in_flight() {
   return NV * V * (int)sizeof(typename T::store) >= 64 ? 2 : NV * V * (int)sizeof(typename T::store) >= 32 ? 4 : 8;
 }
 
+// where a row is, to hand from lane to lane
+template <class S>
+__device__ __forceinline__ u64 lm_address(const S* row) {
+  return (u64) reinterpret_cast<uintptr_t>(row);
+}
+
 // A group takes up to kLmScoreCands candidates of a token: h comes in once for them, their ids with one load (a lane each),
 // their rows several at a time.  The vector unit decides: where a row starts is worked out once, by the lane that loaded the
 // id (a 64-bit product is a dozen full-rate operations), and handed to the group.
@@ -146,6 +160,7 @@ constexpr u32 kLmScoreCands = 16;
 template <class T, int V, int G, int NV, LmRowKind KIND>
 __global__ void __launch_bounds__(kLmThreads)
     k_lm_nce_score(LmNce q, const typename T::store* __restrict__ h, const typename T::store* __restrict__ table, LmIds ids) {
+  typedef typename T::store S;
   constexpr bool BLOCKS = KIND == kLmBlocks, FULL = KIND == kLmFull;
   constexpr int U = BLOCKS ? 1 : lm_rows_in_flight<T, V, NV>();
   const int lane = (int)(threadIdx.x & 63);
@@ -170,32 +185,42 @@ __global__ void __launch_bounds__(kLmThreads)
         hr.mask(0, gl, shape);
       }
       // (an id that names no word reads row 0 for nothing)
-      const u64 atL = rowL < q.vocab ? (u64)rowL * (u64)q.tableStride : 0u;
+      const u64 atL = lm_address(table + (rowL < q.vocab ? (u64)rowL * (u64)q.tableStride : 0u));
       const u32 most = uni(wave_max_u32(cnt));
-      for (u32 k = 0; k < most; k += U) {
-        LmRowPart<T, V, G, NV, FULL> b[U];
-        u64 at[U];
+      // candidates k .. k + R - 1 of every group; k + R <= 16 <= G
+      auto rows = [&](auto many, u32 k) {
+        constexpr u32 R = decltype(many)::value;
+        LmRowPart<T, V, G, NV, FULL> b[R];
+        const S* row[R];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          // (k + u < 16 <= G: kLmScoreCands and U are powers of two)
-          at[u] = wave_shfl_u64(atL, (int)((lane & ~(G - 1)) + k + (u32)u));
-          if constexpr (!BLOCKS) b[u].load(table + at[u], 0, gl, shape);
+        for (u32 u = 0; u < R; ++u) {
+          row[u] = reinterpret_cast<const S*>(wave_shfl_u64(atL, (int)((lane & ~(G - 1)) + k + u)));
+          if constexpr (!BLOCKS) b[u].load(row[u], 0, gl, shape);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (k + (u32)u < most) {
-            float dot;
-            if constexpr (BLOCKS) {
-              dot = lm_dot_blocks<T, V, G, NV>(h + (i64)t * q.hStride, table + at[u], gl, shape);
-            } else {
-              b[u].mask(0, gl, shape);
-              dot = lm_dot_parts<T, V, G, NV, FULL>(hr, b[u]);
-            }
-            dot = lm_group_sum<G>(dot);
-            if (gl == k + (u32)u) mine = dot;
+        for (u32 u = 0; u < R; ++u) {
+          float dot;
+          if constexpr (BLOCKS) {
+            dot = lm_dot_blocks<T, V, G, NV>(h + (i64)t * q.hStride, row[u], gl, shape);
+          } else {
+            b[u].mask(0, gl, shape);
+            dot = lm_dot_parts<T, V, G, NV, FULL>(hr, b[u]);
           }
+          dot = lm_group_sum<G>(dot);
+          mine = gl == k + u ? dot : mine;
         }
+      };
+      u32 k = 0;
+      for (; k + U <= most; k += U) rows(LmConst<U>(), k);
+      if (U > 4 && k + 4 <= most) {
+        rows(LmConst<4>(), k);
+        k += 4;
       }
+      if (U > 2 && k + 2 <= most) {
+        rows(LmConst<2>(), k);
+        k += 2;
+      }
+      if (k < most) rows(LmConst<1>(), k);
     }
     if (gl < cnt) q.out[t * q.cands + k0 + gl] = rowL < q.vocab ? mine - q.constant : -__builtin_inff();
   }
@@ -207,9 +232,10 @@ template <class T, int V, int G, int NV, LmRowKind KIND, bool DH>
 __global__ void __launch_bounds__(kLmThreads)
     k_lm_nce_loss(LmNce q, const typename T::store* __restrict__ h, const typename T::store* __restrict__ table, LmIds ids,
                   typename T::store* __restrict__ dh) {
+  typedef typename T::store S;
   constexpr bool BLOCKS = KIND == kLmBlocks, FULL = KIND == kLmFull;
   constexpr u32 kGroups = 64 / G;
-  constexpr int U = BLOCKS ? 1 : lm_rows_in_flight<T, V, NV>() / 2;
+  constexpr int U = BLOCKS ? 1 : lm_rows_in_flight<T, V, NV>();
   const int lane = (int)(threadIdx.x & 63);
   const u32 gl = threadIdx.x & (G - 1), grp = (u32)lane / G;
   const LmRowShape shape = {q.dim / V, q.dim % V};
@@ -253,44 +279,53 @@ __global__ void __launch_bounds__(kLmThreads)
       const u64 named = wave_ballot(rowL < q.vocab);
       const float biasL = q.constant + lnL;
       // (a candidate that names no word reads the target's row and leaves with a gradient of zero)
-      const u64 atL = (u64)(rowL < q.vocab ? rowL : target) * (u64)q.tableStride;
+      const u64 atL = lm_address(table + (u64)(rowL < q.vocab ? rowL : target) * (u64)q.tableStride);
       // lane k keeps what is candidate k's alone: its logit now, its loss and gradient once for all 64 behind the loop.  In
       // the loop a group makes the gradient of its candidate only as far as dh needs it.
       float zL = 0.f;
-      for (u32 k0 = 0; k0 < kn; k0 += kGroups * U) {
-        LmRowPart<T, V, G, NV, FULL> b[U];
-        u64 at[U];
+      // candidates k0 .. k0 + R kGroups - 1, those behind kn as ones without a word
+      auto rows = [&](auto many, u32 k0) {
+        constexpr u32 R = decltype(many)::value;
+        static_assert(R * kGroups < 64, "a step does not pass the 64th candidate");
+        LmRowPart<T, V, G, NV, FULL> b[R];
+        const S* row[R];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          at[u] = wave_shfl_u64(atL, (int)((k0 + (u32)u * kGroups + grp) & 63));
-          if (!BLOCKS) b[u].load(table + at[u], 0, gl, shape);
+        for (u32 u = 0; u < R; ++u) {
+          row[u] = reinterpret_cast<const S*>(wave_shfl_u64(atL, (int)(k0 + u * kGroups + grp)));
+          if (!BLOCKS) b[u].load(row[u], 0, gl, shape);
         }
         if (kb + k0 == 0) fetch_rest(t + step);
+        constexpr u64 kThese = (u64{1} << (R * kGroups)) - 1;
+        const bool all = ((named >> k0) & kThese) == kThese;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const u32 k = k0 + (u32)u * kGroups + grp;
-          if (k0 + (u32)u * kGroups >= kn) continue;
+        for (u32 u = 0; u < R; ++u) {
+          const u32 k1 = k0 + u * kGroups, k = k1 + grp;
           float dot;
           if constexpr (BLOCKS) {
-            dot = lm_dot_blocks<T, V, G, NV>(h + (i64)t * q.hStride, table + at[u], gl, shape);
+            dot = lm_dot_blocks<T, V, G, NV>(h + (i64)t * q.hStride, row[u], gl, shape);
           } else {
             b[u].mask(0, gl, shape);
             dot = lm_dot_parts<T, V, G, NV, FULL>(hr, b[u]);
           }
-          dot = lm_group_sum<G>(dot);
-          const float bias = wave_shfl_f32(biasL, (int)(k & 63));
-          const float z = dot - bias;
+          const float z = lm_group_sum<G>(dot) - wave_shfl_f32(biasL, (int)k);
           // (lane k of the 64 reads group k mod kGroups)
           const float mine = kGroups == 1 ? z : wave_shfl_f32(z, (int)(((u32)lane & (kGroups - 1)) * G));
-          const u32 k1 = k0 + (u32)u * kGroups;
-          if ((u32)lane >= k1 && (u32)lane < k1 + kGroups) zL = mine;
-          if (DH && !BLOCKS) {
-            float a, c;
-            lm_gate(kb + k == 0 ? -z : z, a, c);
-            if (((named >> (k & 63)) & 1u) != 0) acc.template add<T, G>(kb + k == 0 ? -a * w : a * w, b[u]);
+          zL = (u32)lane - k1 < kGroups ? mine : zL;
+          if constexpr (DH && !BLOCKS) {
+            const float s = kb + k == 0 ? -1.f : 1.f;
+            float gk = lm_row_sigmoid<T>(s * z) * (s * w);
+            if (!all) {   // (a branch around the sum, on its candidates or on their number, has the compiler copy the sum: 16 moves a row)
+              const bool ok = ((named >> k) & 1u) != 0;
+              gk = ok ? gk : 0.f;
+              b[u].keep(ok);
+            }
+            acc.template add<T, G>(gk, b[u]);
           }
         }
-      }
+      };
+      u32 k0 = 0;
+      for (; k0 + kGroups < kn; k0 += kGroups * U) rows(LmConst<U>(), k0);
+      if (k0 < kn) rows(LmConst<1>(), k0);
       const float sign = kb + (u32)lane == 0 ? -1.f : 1.f;
       float sg;
       const float l = lm_softplus(sign * zL, sg);

@@ -140,15 +140,18 @@ def nce_loss(h, table, ids, log_noise, constant, weight, dtype):
     g = sign * sg * w[:, None]
     # sigmoid' = sigmoid (1 - sigmoid) <= sigmoid
     gb = (sg * zb + (GATE + U) * sg) * w[:, None].abs() * ok
+    # the one that 16-bit rows of dh are summed with: exp2(fl(-z fl(log2 e))) within (2 + 1.23 |z|) U, 1 + e, a reciprocal
+    # within 2 U
+    gb_dh = gb if dtype == torch.float32 else gb + 1.3 * z.abs().clamp(max=104) * U * sg * w[:, None].abs() * ok
     live = ok[:, 0]
     hd = torch.where(live[:, None], h.double(), torch.zeros(1, dtype=torch.float64))
     # (a row that does not count may hold anything in the table's or h's place)
     rows = torch.where(ok[:, :, None], rows, torch.zeros(1, dtype=torch.float64))
     zero = torch.zeros(1, dtype=torch.float64)
-    g, gb = torch.where(ok, g, zero), torch.where(ok, gb, zero)
+    g, gb, gb_dh = torch.where(ok, g, zero), torch.where(ok, gb, zero), torch.where(ok, gb_dh, zero)
     loss, loss_b = torch.where(live, loss, zero), torch.where(live, loss_b, zero)
     dh = (g[:, :, None] * rows).sum(1)
-    dh_b = (gb[:, :, None] * rows.abs()).sum(1) + (k + 2) * U * (g.abs()[:, :, None] * rows.abs()).sum(1)
+    dh_b = (gb_dh[:, :, None] * rows.abs()).sum(1) + (k + 2) * U * (g.abs()[:, :, None] * rows.abs()).sum(1)
     entry = (g[:, :, None] * hd[:, None, :]).reshape(-1, dim)
     entry_b = (gb[:, :, None] * hd.abs()[:, None, :]).reshape(-1, dim)
     key = torch.where(ok, ids, torch.full_like(ids, -1)).reshape(-1)
