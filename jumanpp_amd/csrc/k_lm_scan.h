@@ -13,6 +13,10 @@
 //               at the price of reading gate and x (in the gradient gate and dh) twice.
 // The gradient runs backwards: with e the gradient of the state that reaches a row from behind,
 //     delta_t = dh_t + e, dx = delta b, dgate = delta (h_(t-1) - x) a b, e <- a delta.
+// Measured: 16 384 sentences of 31 rows of 128 floats, a wavefront each: 174 us with saved states, 291 us backwards, both
+// 4.6 TB/s (a copy of sets beyond the caches reaches 4.8).  One sentence of 65 536 rows of 1 024 bfloat16 columns in chunks:
+// 55 us for the maps (4.9 TB/s), 6.5 for the states, 68 for the rows (5.9 TB/s).  Walked by one wavefront a column block it
+// takes 19.8 ms.
 // It needs h_(t-1) in 32 bits.  The forward pass leaves the state in front of every kLmSave-th row (an eighth of h's
 // elements); from there the gradient re-makes the states of kLmSave rows in registers, which costs fewer bytes than
 // reading h and does not see h's rounding to 16 bits.
