@@ -359,8 +359,8 @@ u32 scan_pack(u32 dim, i32 type, bool grad) {
 // the sizes alone, not from the type, so that one workspace rule serves all.  Sentences of up to 256 rows are walked, and
 // longer ones where there are enough of about one length to fill the chip: a step of 64 sentences takes 10 us, 44 in chunks;
 // 16 384 sentences of 31 rows take 464 us either way, without the workspace.  Five documents of 40 001 rows of
-// 1 000 columns with the gradient: 206 us in chunks, 6.5 ms walked.  4 096 wavefronts: 3 072 took 3 % longer over 65 536 rows of
-// 1 024 columns, 6 144 and 8 192 6 %.
+// 1 000 columns with the gradient: 206 us in chunks, 6.5 ms walked.  4 096 wavefronts: 6 144 and 8 192 took 6 % longer over 65 536
+// rows of 1 024 columns.
 u32 scan_chunk(u64 rows, u64 n, u64 dim, u64 maxLen) {
   const u64 longest = maxLen == 0 || maxLen > rows ? rows : maxLen;
   const u64 blocks = div_up(dim, 256);
