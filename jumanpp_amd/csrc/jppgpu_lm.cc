@@ -180,10 +180,11 @@ struct SumPlan {
     while ((vocab >> keyBits) != 0) ++keyBits;   // (keys 0 .. vocab)
     passes = (keyBits + 7) / 8;
     one = n <= kLmSortOne;   // (1 003 rows, 100 columns, 30 000 words: 16 us, 25 with the kernels for many)
-    // entries of a thread: eight, or two as long as that makes no more tiles than a workgroup looks back on by itself: 37 us
-    // for the loss of 1 021 tokens, 50 with eight; 309 us for 65 536 tokens, 333 with two (and workgroups of 1 024 threads
-    // took half as long again for their 2.2 M entries)
-    sortRounds = n <= kLmSortOwn * kLmThreads * 2 ? 2 : 8;
+    // entries of a thread: two as long as that makes no more tiles than a workgroup looks back on by itself (37 us for the
+    // loss of 1 021 tokens, 50 with eight), eight where that leaves two workgroups a compute unit (309 us for 65 536 tokens,
+    // 314 with four, 333 with two; workgroups of 1 024 threads took half as long again for their 2.2 M entries), four between
+    // (507 904 ids: 134 us, 139 with eight)
+    sortRounds = n <= kLmSortOwn * kLmThreads * 2 ? 2 : n <= 512u * kLmThreads * 8 ? 4 : 8;
     sortTiles = (u32)div_up(n, kLmThreads * sortRounds);
     // rows that are read again and do not fit one L2: cache lines of 128 bytes spread over the XCDs (k_lm_seg_sum; the step on
     // 65 536 tokens: 309 us, 348 without)
@@ -192,7 +193,7 @@ struct SumPlan {
     lanes = sliced || dim <= 32 ? 8 : dim <= 64 ? 16 : dim <= 128 ? 32 : 64;
     colBlocks = (u32)div_up(div_up(dim, pack), lanes);
     // parts long enough that words rarely cross them, short enough that some eight thousand wavefronts share the work
-    // (507 904 rows: 139 us, 185 in parts of 8; 1 003 rows: 16 us, 27 in parts of 64)
+    // (507 904 rows: a third longer in parts of 8; 1 003 rows: 16 us, 27 in parts of 64)
     part = 8;
     while (part < 64 && (u64)n * div_up(dim, 256) / (part * 2) >= 8192) part *= 2;
     tile = part * (kLmThreads / lanes);
@@ -259,11 +260,15 @@ template <class E, class Keys>
 void sort_pass(Launcher& go, const SumPlan& p, const Keys& keys, u32 shift, u32 bits, const LmZero& zero, E* to) {
   const u64 zeroBlocks = zero_blocks(zero);
   const u32 mask = (1u << bits) - 1;
-  if (p.sortRounds == 2) go(k_lm_sort_count<2, Keys>, p.sortTiles + zeroBlocks, kLmThreads, keys, p.n, shift, mask, p.counts, p.sortTiles, p.spanCount, zero);
-  else go(k_lm_sort_count<8, Keys>, p.sortTiles + zeroBlocks, kLmThreads, keys, p.n, shift, mask, p.counts, p.sortTiles, p.spanCount, zero);
-  if (p.sortTiles > kLmSortOwn) go(k_lm_sort_scan, kLmBins, kLmThreads, p.counts, p.sortTiles, p.totals);
-  if (p.sortRounds == 2) go(k_lm_sort_scatter<2, E, Keys>, p.sortTiles, kLmThreads, keys, p.n, shift, bits, p.counts, p.sortTiles, p.totals, to);
-  else go(k_lm_sort_scatter<8, E, Keys>, p.sortTiles, kLmThreads, keys, p.n, shift, bits, p.counts, p.sortTiles, p.totals, to);
+  auto pass = [&](auto rounds) {
+    constexpr int R = decltype(rounds)::value;
+    go(k_lm_sort_count<R, Keys>, p.sortTiles + zeroBlocks, kLmThreads, keys, p.n, shift, mask, p.counts, p.sortTiles, p.spanCount, zero);
+    if (p.sortTiles > kLmSortOwn) go(k_lm_sort_scan, kLmBins, kLmThreads, p.counts, p.sortTiles, p.totals);
+    go(k_lm_sort_scatter<R, E, Keys>, p.sortTiles, kLmThreads, keys, p.n, shift, bits, p.counts, p.sortTiles, p.totals, to);
+  };
+  if (p.sortRounds == 2) pass(LmConst<2>());
+  else if (p.sortRounds == 4) pass(LmConst<4>());
+  else pass(LmConst<8>());
 }
 
 template <class E>

@@ -11,7 +11,7 @@
 //                                                      crosses parts is put together in LDS, one that crosses tiles leaves a
 //                                                      partial row per tile
 //   k_lm_seg_join                                      the partial rows of those words, in tile order
-// 507 904 bfloat16 rows of 256 columns, 65 521 words: 50 us to sort, 76 to sum, 10 to join.  For the loss, 2.2 M entries on
+// 507 904 bfloat16 rows of 256 columns, 65 521 words: 46 us to sort, 76 to sum, 10 to join.  For the loss, 2.2 M entries on
 // 65 536 such rows: 78, 129 and 5.
 // Rows of words that do not occur are zeroed by workgroups that ride in the grid of the first sorting kernel: that one uses
 // a fraction of the chip.

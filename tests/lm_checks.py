@@ -170,6 +170,30 @@ def embed_grad_words(E, n, kind):
     near(kind, raw_grad(E, E.to(dy), E.to(ids), vocab, 1.0), R.embed_grad(dy, ids, vocab, 1.0))
 
 
+def grad_many(E, n, vocab, dim):
+    g = rng(n)
+    dy, ids = normal(g, n, dim), words(g, vocab, n)
+    got = raw_grad(E, E.to(dy), E.to(ids), vocab, 0.75)
+    near('gradient', got, R.embed_grad(dy, ids, vocab, 0.75))
+    equal('again', raw_grad(E, E.to(dy), E.to(ids), vocab, 0.75), got)
+
+
+@check(case=[(32768, 1000), (32769, 1000), (70003, 70000)])
+def embed_grad_many(E, case):
+    """either side of where a thread of the sort takes more entries, and where the tiles' counts get a kernel of their own"""
+    grad_many(E, *case, 3 if case[0] % 2 else 5)
+
+
+@check('gpu', case=[(300007, 200), (1048576, 60), (1048577, 60), (2000003, 1 << 17)])
+def embed_grad_very_many(E, case):
+    grad_many(E, *case, 6)
+
+
+@check()
+def nce_many(E):
+    one_nce(E, 3001, 11, 500, 5, F32)
+
+
 @check()
 def embed_grad_padding_is_not_read_into_sums(E):
     dy = normal(rng(5), 200, 12)
