@@ -7,6 +7,7 @@ runtime before the library does, which the other GPU tests' process cannot promi
 import json
 import os
 import sys
+import threading
 import traceback
 
 import torch
@@ -706,6 +707,45 @@ def streams(E, big):
     for g, w in zip(got, want):
         for a, b in zip(g, w):
             equal('on a stream', a, b)
+
+
+@check('gpu')
+def threads(E):
+    """threads at once, each on a stream of its own; one that is refused has its own message"""
+    m = [chain_inputs([9, 1, 0, 23, 4] if s % 2 else [900, 40, 700], 40, 36, 5, s) for s in range(4)]
+    want = [chain_step(E, x) for x in m]
+    torch.cuda.synchronize()
+    trouble = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got = chain_step(E, m[i])
+                    torch.cuda.current_stream().synchronize()
+                    for a, b in zip(got, want[i]):
+                        equal('in thread %d' % i, a, b)
+        except Exception:
+            trouble.append(traceback.format_exc())
+
+    def refused():
+        try:
+            for _ in range(50):
+                try:
+                    lm.embed(torch.zeros(3, 4, device='cuda', dtype=BF16), torch.zeros(2, dtype=torch.int32, device='cuda'), dtype=F32)
+                except JppGpuError as e:
+                    assert 'of the table' in str(e), e
+                    continue
+                raise AssertionError('not refused')
+        except Exception:
+            trouble.append(traceback.format_exc())
+
+    running = [threading.Thread(target=work, args=(i,)) for i in range(len(m))] + [threading.Thread(target=refused)]
+    for t in running:
+        t.start()
+    for t in running:
+        t.join()
+    assert not trouble, trouble[0]
 
 
 @check('gpu', big=[False, True])
