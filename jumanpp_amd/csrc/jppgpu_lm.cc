@@ -181,13 +181,13 @@ struct SumPlan {
     passes = (keyBits + 7) / 8;
     one = n <= kLmSortOne;   // (1 003 rows, 100 columns, 30 000 words: 16 us, 25 with the kernels for many)
     // entries of a thread: two as long as that makes no more tiles than a workgroup looks back on by itself (37 us for the
-    // loss of 1 021 tokens, 50 with eight), eight where that leaves two workgroups a compute unit (309 us for 65 536 tokens,
-    // 314 with four, 333 with two; workgroups of 1 024 threads took half as long again for their 2.2 M entries), four between
-    // (507 904 ids: 134 us, 139 with eight)
+    // loss of 1 021 tokens, 50 with eight), eight where that leaves two workgroups a compute unit (2.2 M entries: 5 us more
+    // with four, 24 with two; in workgroups of 1 024 threads half as long again), four between (507 904 ids: 5 us less than
+    // with eight)
     sortRounds = n <= kLmSortOwn * kLmThreads * 2 ? 2 : n <= 512u * kLmThreads * 8 ? 4 : 8;
     sortTiles = (u32)div_up(n, kLmThreads * sortRounds);
     // rows that are read again and do not fit one L2: cache lines of 128 bytes spread over the XCDs (k_lm_seg_sum; the step on
-    // 65 536 tokens: 309 us, 348 without)
+    // 65 536 tokens: 300 us, 39 more without)
     const bool sliced = perToken > 1 && dim >= 64 && n / perToken * dim * 2 > kL2Bytes;
     pack = dim < 4 ? 1 : sliced && bytes_of(type) == 2 ? 8 : 4;
     lanes = sliced || dim <= 32 ? 8 : dim <= 64 ? 16 : dim <= 128 ? 32 : 64;

@@ -11,10 +11,11 @@
 //                                                      crosses parts is put together in LDS, one that crosses tiles leaves a
 //                                                      partial row per tile
 //   k_lm_seg_join                                      the partial rows of those words, in tile order
-// 507 904 bfloat16 rows of 256 columns, 65 521 words: 46 us to sort, 76 to sum, 10 to join.  For the loss, 2.2 M entries on
-// 65 536 such rows: 78, 129 and 5.
+// 507 904 bfloat16 rows of 256 columns, 65 521 words: 44 us to sort, 73 to sum, 9 to join.
+// For the loss, 2.2 M entries on 65 536 such rows: 74, 128 and 5.
 // Rows of words that do not occur are zeroed by workgroups that ride in the grid of the first sorting kernel: that one uses
-// a fraction of the chip.
+// a fraction of the chip.  Zeros and finished rows leave with the non-temporal hint: the gradient is not read here, src is
+// (134 us without for the lookup's gradient above, 126 with; small ones are within 1 % either way).
 #ifndef JPP_K_LM_EMBED_H
 #define JPP_K_LM_EMBED_H
 
@@ -79,7 +80,7 @@ __device__ __forceinline__ void lm_zero_rows(const LmZero& z, u64 first, u64 ste
     const u32 packs = cols / 4;
     LmPack<LmF32, 4> zero;
     zero.zero();
-    for (u32 c = threadIdx.x; c < packs; c += blockDim.x) lm_store<LmF32, 4>(row + 4 * (u64)c, zero);
+    for (u32 c = threadIdx.x; c < packs; c += blockDim.x) lm_store<LmF32, 4, true>(row + 4 * (u64)c, zero);
     for (u32 c = packs * 4 + threadIdx.x; c < cols; c += blockDim.x) row[c] = 0.f;
   }
 }
@@ -395,7 +396,7 @@ struct LmSeg {
 // most of which its own L2 then holds (half lines, eight blocks of 256 columns of bf16, were no use: the L2 fetches whole
 // ones).  The loss of 65 536 tokens: 1.1 GB of rows through the L2s in 129 us, of which 0.75 GB come from outside them, which
 // is what bounds it; with whole rows a group the step takes 39 us longer.  The lookup's gradient reads 260 MB and writes
-// 67 MB in 76 us: 4.3 TB/s.
+// 67 MB in 73 us: 4.5 TB/s.
 template <class T, int V, int L, class E>
 __global__ void __launch_bounds__(kLmThreads) k_lm_seg_sum(LmSeg<E> q, const typename T::store* __restrict__ src) {
   constexpr int kGroups = kLmThreads / L, kCols = L * V;
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_seg_sum(LmSeg<E> q, const typ
                   for (int e = 0; e < V; ++e) s_head[grp][gl * V + (u32)e] = acc[e];
                   flags |= 1;
                 } else if (on) {
-                  lm_store<LmF32, V>(q.grad + (i64)cur * q.gradStride + col, lm_pack<LmF32, V>(acc));
+                  lm_store<LmF32, V, true>(q.grad + (i64)cur * q.gradStride + col, lm_pack<LmF32, V>(acc));
                 }
               }
               first = false;
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_seg_sum(LmSeg<E> q, const typ
           for (int e = 0; e < V; ++e) s_tail[grp][gl * V + (u32)e] = acc[e];
           flags |= 4;
         } else if (on) {
-          lm_store<LmF32, V>(q.grad + (i64)cur * q.gradStride + col, lm_pack<LmF32, V>(acc));
+          lm_store<LmF32, V, true>(q.grad + (i64)cur * q.gradStride + col, lm_pack<LmF32, V>(acc));
         }
       }
     }
@@ -519,7 +520,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_seg_sum(LmSeg<E> q, const typ
 
 // A word over several tiles: tail of the first, heads of the following ones.  A workgroup takes 64 V columns of a word; its
 // wavefronts take consecutive parts of the tiles, and their sums are added in that order.  Latency bounds it: the list, the
-// key, the tiles' keys, their rows, one after the other (a word of every fifteenth of 507 904 rows is 264 tiles: 10 us; 13
+// key, the tiles' keys, their rows, one after the other (a word of every fifteenth of 507 904 rows is 264 tiles: 9 us; 13
 // with a column a lane).
 constexpr int kLmJoinWaves = 4;
 template <int V, class E>

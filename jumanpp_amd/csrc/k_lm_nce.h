@@ -7,13 +7,13 @@
 // The rows of W are gathered: the bytes of K rows a token decide, from L2 and the memory-side cache for a table that fits
 // there.  A group of G lanes holds a row in registers, so the loss reads every row once -- the product with h, then
 // g_k times the same registers into dh.  G = 16 keeps the product's reduction inside a row of 16 lanes (four DPP steps,
-// four candidates side by side); longer rows take the whole wavefront (for 256 columns of 16 bits that takes the step 535 us
-// in place of 309: a reduction over 64 lanes for every candidate, none side by side).
+// four candidates side by side); longer rows take the whole wavefront (for 256 columns of 16 bits the loss would take three
+// times as long: a reduction over 64 lanes for every candidate, none side by side).
 // 507 904 tokens, 6 candidates, 128 bfloat16 columns are scored in 57 us: 0.72 GB asked of the L2s, 0.28 GB of it from outside,
 // the vector unit taking 0.6 of its slots.  The loss of 65 536 tokens, 33 candidates, 256 columns takes 107 us with dh, the
 // vector unit 0.74 of its slots: that is the bound there.  Hence the products in pairs (lm_dot2), addresses made once and
-// handed on, and the exact row length as a kind of its own: 57 us against 70 with the masks of shorter rows, 309 against 344
-// for the step.
+// handed on, and the exact row length as a kind of its own: 57 us against 70 with the masks of shorter rows; the loss gains
+// 35 us.
 #ifndef JPP_K_LM_NCE_H
 #define JPP_K_LM_NCE_H
 
