@@ -217,28 +217,64 @@ __device__ __forceinline__ void lm_gate(float z, float& a, float& b) {
   b = up ? er : r;
 }
 
-// The gate of a row of T.  A 16-bit row's outputs are rounded to 2^-12 or 2^-9, and the vector unit takes longer over a gate
-// than memory over its element: there without the corrections (exp within (3 + 1.3 |z|) 2^-24 of itself, the reciprocal
-// within 2^-23; the states these gates make stay 32 bits).
+// A gate as the smaller of sigmoid(z) and sigmoid(-z), with the sign of z: a step's weights are it and what it leaves of one, so
+// they sum to one however they are rounded.  (Rounded apart, they miss it by up to 2^-24, and a state that is a mean over
+// 1 / (1 - a) rows shows that as many times over: 3e-4 of itself behind 40 000 gates of 10.)
+// A 16-bit row's outputs are rounded to 2^-12 or 2^-9, and the vector unit takes longer over a gate than memory over its element:
+// there without the corrections (exp within (3 + 1.3 |z|) 2^-24 of itself, the reciprocal within 2^-23).
 template <class T>
-__device__ __forceinline__ void lm_row_gate(float z, float& a, float& b) {
+__device__ __forceinline__ float lm_row_weight(float z) {
+  float e, r;
   if constexpr (sizeof(typename T::store) == 4) {
-    lm_gate(z, a, b);
+    e = lm_exp_neg(__builtin_fabsf(z));
+    r = lm_rcp(1.f + e);
   } else {
-    const float e = lm_exp2(-__builtin_fabsf(z) * 1.44269504088896341f);
+    e = lm_exp2(-__builtin_fabsf(z) * 1.44269504088896341f);
 #if defined(__HIP_DEVICE_COMPILE__)
-    const float r = __builtin_amdgcn_rcpf(1.f + e);
+    r = __builtin_amdgcn_rcpf(1.f + e);
 #else
-    const float r = 1.f / (1.f + e);
+    r = 1.f / (1.f + e);
 #endif
-    const float er = e * r;
-    const bool up = z >= 0.f;
-    a = up ? r : er;
-    b = up ? er : r;
   }
+  return __builtin_copysignf(e * r, z);
+}
+__device__ __forceinline__ bool lm_open(float w) { return (i32)LmF32::put(w) >= 0; }   // (a weight may be a zero with a sign)
+// a v + (1 - a) x, from the larger weight's side
+__device__ __forceinline__ float lm_step(float w, float v, float x) { return __builtin_fmaf(w, x - v, lm_open(w) ? v : x); }
+// a v and (1 - a) v
+__device__ __forceinline__ float lm_kept(float w, float v) { return __builtin_fmaf(-w, v, lm_open(w) ? v : 0.f); }
+__device__ __forceinline__ float lm_let_in(float w, float v) { return __builtin_fmaf(w, v, lm_open(w) ? 0.f : v); }
+// The same from the two weights, for states that are not finite, or further than the largest number from what comes in: there
+// differences are NaN or infinite where the formula's value is not.
+struct LmWeights {
+  float a, b;
+  __device__ __forceinline__ explicit LmWeights(float w) {
+    const float s = __builtin_fabsf(w), l = 1.f - s;
+    a = lm_open(w) ? l : s;
+    b = lm_open(w) ? s : l;
+  }
+};
+__device__ __forceinline__ bool lm_finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
+
+// Many steps are v -> A v + B.  Their A is held like a gate's weights, and for the same reason (the same sentence may have the same
+// gates in every chunk, and the same rounding of their product): 1 - A, or - A where that is the smaller.  kLmFresh: nothing of v
+// passes, also where v is no number.
+constexpr float kLmFresh = -2.f;
+__device__ __forceinline__ float lm_map_weight(float A, float C) { return C <= 0.5f ? C : -A; }   // C: 1 - A, made for itself
+// the map of weight w2 behind that of weight w1
+__device__ __forceinline__ float lm_map_weight_then(float w1, float w2) {
+  const float A1 = lm_open(w1) ? 1.f - w1 : -w1, C1 = lm_open(w1) ? w1 : 1.f + w1;
+  const float w = lm_map_weight(lm_kept(w2, A1), lm_step(w2, C1, 1.f));
+  return w1 == kLmFresh || w2 == kLmFresh ? kLmFresh : w;
+}
+__device__ __forceinline__ float lm_map(float w, float v, float B) {
+  float r = __builtin_fmaf(-w, v, B) + (lm_open(w) ? v : 0.f);
+  // (A is never zero, though its product may be: an infinity passes)
+  if (!lm_finite(r)) r = lm_finite(v) ? __builtin_fmaf(lm_open(w) ? 1.f - w : -w, v, B) : v + B;
+  return w == kLmFresh ? B : r;
 }
 
-// sigmoid(z), as far as rows of T show it: for 16 bits within (5 + 1.3 |z|) 2^-24 of itself, for the reasons of lm_row_gate
+// sigmoid(z), as far as rows of T show it: for 16 bits within (5 + 1.3 |z|) 2^-24 of itself, for the reasons of lm_row_weight
 template <class T>
 __device__ __forceinline__ float lm_row_sigmoid(float z) {
   if constexpr (sizeof(typename T::store) == 4) {

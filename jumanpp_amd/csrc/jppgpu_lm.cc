@@ -386,7 +386,7 @@ void launch_scan(Launcher& go, const LmScan<T>& q) {
   }
   const u64 blocks = div_up((u64)q.chunks * q.colBlocks, waves), groups = div_up(q.chunks, kLmGroup) * q.colBlocks;
   go(k_lm_scan_agg<T, V>, groups, kLmThreads, q);
-  go(k_lm_scan_carry<false>, div_up(q.dim, kLmCarryCols), kLmCarryCols * kLmCarryRuns, q.groupA, q.groupB, (u32)div_up(q.chunks, kLmGroup), q.dim);
+  go(k_lm_scan_carry<false>, div_up(q.dim, kLmCarryCols), kLmCarryCols * kLmCarryRuns, q.groupW, q.groupB, (u32)div_up(q.chunks, kLmGroup), q.dim);
   if (q.saved != nullptr) go(k_lm_scan_chunk<T, V, true, STREAM>, blocks, kLmThreads, q);
   else go(k_lm_scan_chunk<T, V, false, STREAM>, blocks, kLmThreads, q);
 }
@@ -400,7 +400,7 @@ void launch_scan_grad(Launcher& go, const LmScan<T>& q) {
   }
   const u64 blocks = div_up((u64)q.chunks * q.colBlocks, waves), groups = div_up(q.chunks, kLmGroup) * q.colBlocks;
   go(k_lm_scan_grad_agg<T, V>, groups, kLmThreads, q);
-  go(k_lm_scan_carry<true>, div_up(q.dim, kLmCarryCols), kLmCarryCols * kLmCarryRuns, q.groupA, q.groupB, (u32)div_up(q.chunks, kLmGroup), q.dim);
+  go(k_lm_scan_carry<true>, div_up(q.dim, kLmCarryCols), kLmCarryCols * kLmCarryRuns, q.groupW, q.groupB, (u32)div_up(q.chunks, kLmGroup), q.dim);
   go(k_lm_scan_grad_chunk<T, V, STREAM>, blocks, kLmThreads, q);
 }
 
@@ -416,10 +416,10 @@ void launch_scan_any(Launcher& go, const LmScan<T>& q, bool grad) {
   }
 }
 
-void carve_maps(Carver& c, u64 chunks, u64 dim, float** aggA, float** aggB, float** groupA, float** groupB) {
-  *aggA = c.take<float>(chunks * dim);
+void carve_maps(Carver& c, u64 chunks, u64 dim, float** aggW, float** aggB, float** groupW, float** groupB) {
+  *aggW = c.take<float>(chunks * dim);
   *aggB = c.take<float>(chunks * dim);
-  *groupA = c.take<float>(div_up(chunks, kLmGroup) * dim);
+  *groupW = c.take<float>(div_up(chunks, kLmGroup) * dim);
   *groupB = c.take<float>(div_up(chunks, kLmGroup) * dim);
 }
 
@@ -477,7 +477,7 @@ void run_scan(Launcher& go, const ScanArgs& s, bool grad) {
   if (q.chunk != 0) {
     q.chunks = (u32)div_up(q.rows, q.chunk);
     Carver c{static_cast<char*>(s.workspace)};
-    carve_maps(c, q.chunks, q.dim, &q.aggA, &q.aggB, &q.groupA, &q.groupB);
+    carve_maps(c, q.chunks, q.dim, &q.aggW, &q.aggB, &q.groupW, &q.groupB);
   }
   if (v == 1) launch_scan_any<T, 1>(go, q, grad);
   else if (v == 2) launch_scan_any<T, 2>(go, q, grad);

@@ -5,12 +5,14 @@
 // decide.  Two splits:
 //   short sentences (k_lm_scan_seq, k_lm_scan_grad_seq)  a wavefront per sentence and column block, one pass over the data;
 //   long ones   the packed rows in chunks of C rows, whatever sentences they belong to.  A chunk maps the state in front of
-//               it to the state behind it by s -> A s + B, or to B alone where a sentence begins inside (A = -1 says so: 0 s
-//               would let a NaN of one sentence into the next):
+//               it to the state behind it by s -> A s + B, or to B alone where a sentence begins inside:
 //                 k_lm_scan_agg, k_lm_scan_grad_agg   A and B of every chunk, put together in groups of four
 //                 k_lm_scan_carry                     the states between the groups
 //                 k_lm_scan_chunk, k_lm_scan_grad_chunk   the rows themselves, from the states
 //               at the price of reading gate and x (in the gradient gate and dh) twice.
+// A row's step is made from the smaller of its two weights, s (jpp_lm.h): h_t = h_(t-1) + s (x_t - h_(t-1)), or from x_t's side,
+// so that the weights sum to one and no rounding of a weight is gathered up over a long memory.  A state that is not a number
+// afterwards, every eight rows, has them made again from the two weights, which is what the formula says of infinities.
 // The gradient runs backwards: with e the gradient of the state that reaches a row from behind,
 //     delta_t = dh_t + e, dx = delta b, dgate = delta (h_(t-1) - x) a b, e <- a delta.
 // Measured: 16 384 sentences of 31 rows of 128 floats, a wavefront each: 174 us with saved states, 291 us backwards, both
@@ -56,8 +58,8 @@ struct LmScan {
   i64 dstateStride;
   // chunks
   u32 chunk, chunks;      // rows of a chunk (a multiple of kLmSave), chunks
-  float *aggA, *aggB;     // [chunks][dim] map of the chunks of its group that lie in front of a chunk
-  float *groupA, *groupB; // [groups][dim] map of a group of kLmGroup chunks; k_lm_scan_carry turns B into the state that enters it
+  float *aggW, *aggB;     // [chunks][dim] map of the chunks of its group that lie in front of a chunk
+  float *groupW, *groupB; // [groups][dim] map of a group of kLmGroup chunks; k_lm_scan_carry turns B into the state that enters it
 };
 constexpr u32 kLmGroup = kLmThreads / 64;   // chunks that a workgroup of the aggregating kernels takes, a wavefront each
 
@@ -100,6 +102,34 @@ __device__ __forceinline__ void lm_put_f32(float* base, i64 stride, u32 row, u32
   lm_store<LmF32, V>(base + (i64)row * stride + col, lm_pack<LmF32, V>(v));
 }
 
+// Rows [r0, r1) of one sentence, forward, from state v, by the two weights: for the elements of a pack that are `odd`, the others
+// as ever (two lanes may share a column).  STORE: h too.  Rare, so nothing is held or unrolled for it.
+template <class T, int V, bool STORE, bool STREAM>
+__device__ __forceinline__ void lm_scan_rows_weights(const LmScan<T>& q, u32 r0, u32 r1, u32 col, const bool (&odd)[V], float (&v)[V]) {
+#pragma unroll 1
+  for (u32 r = r0; r < r1; ++r) {
+    const LmPack<T, V> f = lm_load<T, V>(q.gate + (i64)r * q.gateStride + col), x = lm_load<T, V>(q.x + (i64)r * q.xStride + col);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float w = lm_row_weight<T>(f.get(e));
+      const LmWeights p(w);
+      v[e] = odd[e] ? __builtin_fmaf(p.a, v[e], p.b * x.get(e)) : lm_step(w, v[e], x.get(e));
+    }
+    if constexpr (STORE) lm_store<T, V, STREAM>(q.h + (i64)r * q.hStride + col, lm_pack<T, V>(v));
+  }
+}
+// which elements are not numbers (a state that is none stays so to the end of its sentence)
+template <int V>
+__device__ __forceinline__ bool lm_odd(const float (&v)[V], bool (&odd)[V]) {
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    odd[e] = !lm_finite(v[e]);
+    any = any || odd[e];
+  }
+  return any;
+}
+
 // Rows [r0, r1) of one sentence, forward, from state v.
 template <class T, int V, bool SAVE, bool STREAM>
 __device__ __forceinline__ void lm_scan_rows(const LmScan<T>& q, u32 r0, u32 r1, u32 col, float (&v)[V]) {
@@ -114,19 +144,50 @@ __device__ __forceinline__ void lm_scan_rows(const LmScan<T>& q, u32 r0, u32 r1,
       x[i] = lm_load<T, V>(q.x + (i64)r * q.xStride + col);
     }
     if (SAVE && t % kLmSave == 0) lm_put_f32<V>(q.saved, q.dim, t / kLmSave, col, v);
+    float v0[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v0[e] = v[e];
 #pragma unroll
     for (u32 i = 0; i < kLmSave; ++i) {
       if (i < cnt) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float a, b;
-          lm_row_gate<T>(f[i].get(e), a, b);
-          v[e] = __builtin_fmaf(a, v[e], b * x[i].get(e));
-        }
+        for (int e = 0; e < V; ++e) v[e] = lm_step(lm_row_weight<T>(f[i].get(e)), v[e], x[i].get(e));
         lm_store<T, V, STREAM>(q.h + (i64)(t + i) * q.hStride + col, lm_pack<T, V>(v));
       }
     }
+    bool odd[V];
+    if (lm_odd<V>(v, odd)) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = v0[e];
+      lm_scan_rows_weights<T, V, true, STREAM>(q, t, t + cnt, col, odd, v);
+    }
     t += cnt;
+  }
+}
+
+// Rows [r0, r1), at most kLmSave of them from a sentence's first or a saved one on, backward, by the two weights (see
+// lm_scan_rows_weights): the state in front of every row is walked to anew.
+template <class T, int V, bool STREAM>
+__device__ __forceinline__ void lm_scan_grad_rows_weights(const LmScan<T>& q, u32 sentence, u32 begin, u32 r0, u32 r1, u32 col,
+                                                          const bool (&odd)[V], float (&e)[V]) {
+#pragma unroll 1
+  for (u32 r = r1; r-- > r0;) {
+    float v[V], df[V], dx[V];
+    if (r0 == begin) lm_row_f32<V>(q.state, q.stateStride, sentence, col, v);
+    else lm_row_f32<V>(q.saved, q.dim, r0 / kLmSave, col, v);
+    lm_scan_rows_weights<T, V, false, STREAM>(q, r0, r, col, odd, v);
+    const LmPack<T, V> f = lm_load<T, V>(q.gate + (i64)r * q.gateStride + col), x = lm_load<T, V>(q.x + (i64)r * q.xStride + col);
+    const LmPack<T, V> d = lm_load<T, V>(q.dh + (i64)r * q.dhStride + col);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float w = lm_row_weight<T>(f.get(k)), delta = d.get(k) + e[k], s = __builtin_fabsf(w);
+      const LmWeights p(w);
+      dx[k] = odd[k] ? p.b * delta : lm_let_in(w, delta);
+      e[k] = odd[k] ? p.a * delta : lm_kept(w, delta);
+      df[k] = delta * __builtin_fmaf(-s, s, s) * (v[k] - x.get(k));
+    }
+    lm_store<T, V, STREAM>(q.dgate + (i64)r * q.dgateStride + col, lm_pack<T, V>(df));
+    lm_store<T, V, STREAM>(q.dx + (i64)r * q.dxStride + col, lm_pack<T, V>(dx));
   }
 }
 
@@ -147,18 +208,20 @@ __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 senten
       d[i] = lm_load<T, V>(q.dh + (i64)r * q.dhStride + col);
     }
     // the state in front of row t: t is the sentence's first row or a saved one (chunks begin on saved rows)
-    float v[V], before[kLmSave][V], a[kLmSave][V], b[kLmSave][V];
+    float v[V], before[kLmSave][V], w[kLmSave][V], e1[V];
     if (t == begin) lm_row_f32<V>(q.state, q.stateStride, sentence, col, v);
     else lm_row_f32<V>(q.saved, q.dim, t / kLmSave, col, v);
 #pragma unroll
     for (u32 i = 0; i < kLmSave; ++i) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        lm_row_gate<T>(f[i].get(k), a[i][k], b[i][k]);
+        w[i][k] = lm_row_weight<T>(f[i].get(k));
         before[i][k] = v[k];
-        v[k] = __builtin_fmaf(a[i][k], v[k], b[i][k] * x[i].get(k));
+        v[k] = lm_step(w[i][k], v[k], x[i].get(k));
       }
     }
+#pragma unroll
+    for (int k = 0; k < V; ++k) e1[k] = e[k];
 #pragma unroll
     for (u32 j = 0; j < kLmSave; ++j) {
       const u32 i = kLmSave - 1 - j;
@@ -166,14 +229,24 @@ __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 senten
         float df[V], dx[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float delta = d[i].get(k) + e[k];
-          dx[k] = delta * b[i][k];
-          e[k] = delta * a[i][k];
-          df[k] = dx[k] * (before[i][k] - x[i].get(k)) * a[i][k];
+          const float delta = d[i].get(k) + e[k], s = __builtin_fabsf(w[i][k]);
+          dx[k] = lm_let_in(w[i][k], delta);
+          e[k] = lm_kept(w[i][k], delta);
+          df[k] = delta * __builtin_fmaf(-s, s, s) * (before[i][k] - x[i].get(k));   // (a b = s (1 - s))
         }
         lm_store<T, V, STREAM>(q.dgate + (i64)(t + i) * q.dgateStride + col, lm_pack<T, V>(df));
         lm_store<T, V, STREAM>(q.dx + (i64)(t + i) * q.dxStride + col, lm_pack<T, V>(dx));
       }
+    }
+    bool odd[V], oddV[V];
+    const bool oddE = lm_odd<V>(e, odd);
+    if (lm_odd<V>(v, oddV) || oddE) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        odd[k] = odd[k] || oddV[k];
+        e[k] = e1[k];
+      }
+      lm_scan_grad_rows_weights<T, V, STREAM>(q, sentence, begin, t, end, col, odd, e);
     }
     end = t;
   }
@@ -214,56 +287,78 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_seq(LmScan<T> q) {
 
 // ---- chunks ------------------------------------------------------------------------
 template <int V>
-struct LmMap {   // s -> A s + B, or B where A < 0
-  float A[V], B[V];
+struct LmMap {   // s -> A s + B; W: the weight of A (lm_map_weight)
+  float W[V], B[V];
+  __device__ __forceinline__ void one() {
+#pragma unroll
+    for (int e = 0; e < V; ++e) W[e] = B[e] = 0.f;
+  }
+  // this map, then the map (w, b)
+  __device__ __forceinline__ void then(int e, float w, float b) {
+    B[e] = lm_map(w, B[e], b);
+    W[e] = lm_map_weight_then(W[e], w);
+  }
+};
+// ... of rows, made row by row
+template <int V>
+struct LmRowsMap {
+  float A[V], C[V], B[V];   // C = 1 - A
   __device__ __forceinline__ void one() {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       A[e] = 1.f;
-      B[e] = 0.f;
+      C[e] = B[e] = 0.f;
     }
   }
-  // this map, then the map (a, b)
-  __device__ __forceinline__ void then(int e, float a, float b) {
-    B[e] = a < 0.f ? b : __builtin_fmaf(a, B[e], b);
-    A[e] = a < 0.f || A[e] < 0.f ? -1.f : A[e] * a;
+  __device__ __forceinline__ void pass(int e, float w) {
+    A[e] = lm_kept(w, A[e]);
+    C[e] = lm_step(w, C[e], 1.f);
+  }
+  __device__ __forceinline__ LmMap<V> map(bool fresh) const {
+    LmMap<V> m;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      m.W[e] = fresh ? kLmFresh : lm_map_weight(A[e], C[e]);
+      m.B[e] = B[e];
+    }
+    return m;
   }
 };
 
 // The maps of a workgroup's chunks, a wavefront each: what lies in front of a chunk inside the group, and the group's own.
 // BACK: in front is behind.
 template <int V, bool BACK>
-__device__ __forceinline__ void lm_scan_group(LmMap<V>& m, float (&sA)[kLmGroup][64 * V], float (&sB)[kLmGroup][64 * V], float* aggA, float* aggB,
-                                              float* groupA, float* groupB, u32 group, u32 chunk, u32 chunks, u32 dim, u32 col, int lane, int wv) {
+__device__ __forceinline__ void lm_scan_group(LmMap<V> m, float (&sW)[kLmGroup][64 * V], float (&sB)[kLmGroup][64 * V], float* aggW, float* aggB,
+                                              float* groupW, float* groupB, u32 group, u32 chunk, u32 chunks, u32 dim, u32 col, int lane, int wv) {
   // order of the walk
   const int at = BACK ? (int)kLmGroup - 1 - wv : wv;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    sA[at][lane * V + e] = m.A[e];
+    sW[at][lane * V + e] = m.W[e];
     sB[at][lane * V + e] = m.B[e];
   }
   __syncthreads();
   m.one();
   for (int w = 0; w < at; ++w)
 #pragma unroll
-    for (int e = 0; e < V; ++e) m.then(e, sA[w][lane * V + e], sB[w][lane * V + e]);
+    for (int e = 0; e < V; ++e) m.then(e, sW[w][lane * V + e], sB[w][lane * V + e]);
   if (chunk < chunks) {
-    lm_put_f32<V>(aggA, dim, chunk, col, m.A);
+    lm_put_f32<V>(aggW, dim, chunk, col, m.W);
     lm_put_f32<V>(aggB, dim, chunk, col, m.B);
   }
   if (at == (int)kLmGroup - 1) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) m.then(e, sA[at][lane * V + e], sB[at][lane * V + e]);
-    lm_put_f32<V>(groupA, dim, group, col, m.A);
+    for (int e = 0; e < V; ++e) m.then(e, sW[at][lane * V + e], sB[at][lane * V + e]);
+    lm_put_f32<V>(groupW, dim, group, col, m.W);
     lm_put_f32<V>(groupB, dim, group, col, m.B);
   }
   __syncthreads();
 }
 
-// state behind the chunk = A * state in front of it + B
+// state behind the chunk = A state in front of it + B
 template <class T, int V>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_agg(LmScan<T> q) {
-  __shared__ float s_A[kLmGroup][64 * V], s_B[kLmGroup][64 * V];
+  __shared__ float s_W[kLmGroup][64 * V], s_B[kLmGroup][64 * V];
   const int lane = (int)(threadIdx.x & 63), wv = (int)(threadIdx.x >> 6);
   const u32 packs = (q.dim + V - 1) / V;
   const u64 blocks = (u64)((q.chunks + kLmGroup - 1) / kLmGroup) * q.colBlocks;
@@ -272,13 +367,13 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_agg(LmScan<T> q) {
     // (lanes behind the last column repeat it: the same loads, the same stores)
     const u32 pack = cb * 64u + (u32)lane;
     const u32 col = lm_col<V>(pack < packs ? pack : packs - 1, q.dim);
-    LmMap<V> m;
+    LmRowsMap<V> m;
     m.one();
+    bool fresh = false;   // nothing passes
     if (c < q.chunks) {
       const u32 r0 = c * q.chunk, r1 = q.rows - r0 < q.chunk ? q.rows : r0 + q.chunk;
       // only the sentence that holds the chunk's last row reaches past it
       const u32 i = uni(lm_sentence_of(q.offsets, q.n, r1 - 1, lane));
-      bool fresh = false;   // nothing passes
       u32 from = r0, to = r0;
       if (i < q.n) {
         const u32 begin = lm_offset(q.offsets, i, q.rows), end = lm_offset(q.offsets, i + 1, q.rows);
@@ -296,30 +391,36 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_agg(LmScan<T> q) {
           f[k] = lm_load<T, V>(q.gate + (i64)r * q.gateStride + col);
           x[k] = lm_load<T, V>(q.x + (i64)r * q.xStride + col);
         }
+        float B0[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) B0[e] = m.B[e];
 #pragma unroll
         for (u32 k = 0; k < kLmSave; ++k) {
           if (k < cnt) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              float a, b;
-              lm_row_gate<T>(f[k].get(e), a, b);
-              m.A[e] *= a;
-              m.B[e] = __builtin_fmaf(a, m.B[e], b * x[k].get(e));
+              const float w = lm_row_weight<T>(f[k].get(e));
+              m.pass(e, w);
+              m.B[e] = lm_step(w, m.B[e], x[k].get(e));
             }
           }
         }
-      }
+        bool odd[V];
+        if (lm_odd<V>(m.B, odd)) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) m.A[e] = fresh ? -1.f : m.A[e];
+          for (int e = 0; e < V; ++e) m.B[e] = B0[e];
+          lm_scan_rows_weights<T, V, false, false>(q, t, cnt < kLmSave ? to : t + kLmSave, col, odd, m.B);
+        }
+      }
     }
-    lm_scan_group<V, false>(m, s_A, s_B, q.aggA, q.aggB, q.groupA, q.groupB, g, c, q.chunks, q.dim, col, lane, wv);
+    lm_scan_group<V, false>(m.map(fresh), s_W, s_B, q.aggW, q.aggB, q.groupW, q.groupB, g, c, q.chunks, q.dim, col, lane, wv);
   }
 }
 
-// gradient of the state in front of the chunk = A * gradient of the state behind it + B
+// gradient of the state in front of the chunk = A gradient of the state behind it + B
 template <class T, int V>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
-  __shared__ float s_A[kLmGroup][64 * V], s_B[kLmGroup][64 * V];
+  __shared__ float s_W[kLmGroup][64 * V], s_B[kLmGroup][64 * V];
   const int lane = (int)(threadIdx.x & 63), wv = (int)(threadIdx.x >> 6);
   const u32 packs = (q.dim + V - 1) / V;
   const u64 blocks = (u64)((q.chunks + kLmGroup - 1) / kLmGroup) * q.colBlocks;
@@ -327,13 +428,13 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
     const u32 g = (u32)(block / q.colBlocks), cb = (u32)(block - (u64)g * q.colBlocks), c = g * kLmGroup + (u32)wv;
     const u32 pack = cb * 64u + (u32)lane;
     const u32 col = lm_col<V>(pack < packs ? pack : packs - 1, q.dim);
-    LmMap<V> m;
+    LmRowsMap<V> m;
     m.one();
+    bool fresh = false;   // nothing passes
     if (c < q.chunks) {
       const u32 r0 = c * q.chunk, r1 = q.rows - r0 < q.chunk ? q.rows : r0 + q.chunk;
       // only the sentence that holds the chunk's first row reaches in front of it
       const u32 i = uni(lm_sentence_of(q.offsets, q.n, r0, lane));
-      bool fresh = false;   // nothing passes
       u32 to = r0;
       if (i < q.n) {
         const u32 end = lm_offset(q.offsets, i + 1, q.rows);
@@ -351,37 +452,52 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
           f[k] = lm_load<T, V>(q.gate + (i64)r * q.gateStride + col);
           d[k] = lm_load<T, V>(q.dh + (i64)r * q.dhStride + col);
         }
+        float B0[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) B0[e] = m.B[e];
 #pragma unroll
         for (u32 j = 0; j < kLmSave; ++j) {
           const u32 k = kLmSave - 1 - j;
           if (k < cnt) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              float a, b;
-              lm_row_gate<T>(f[k].get(e), a, b);
-              m.A[e] *= a;
-              m.B[e] = a * (m.B[e] + d[k].get(e));
+              const float w = lm_row_weight<T>(f[k].get(e));
+              m.pass(e, w);
+              m.B[e] = lm_kept(w, m.B[e] + d[k].get(e));
             }
           }
         }
+        bool odd[V];
+        if (lm_odd<V>(m.B, odd)) {
+#pragma unroll 1
+          for (u32 r = end; r-- > t;) {
+            const LmPack<T, V> g = lm_load<T, V>(q.gate + (i64)r * q.gateStride + col), u = lm_load<T, V>(q.dh + (i64)r * q.dhStride + col);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float w = lm_row_weight<T>(g.get(e));
+              B0[e] += u.get(e);
+              B0[e] = odd[e] ? LmWeights(w).a * B0[e] : lm_kept(w, B0[e]);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) m.B[e] = B0[e];
+        }
         end = t;
       }
-#pragma unroll
-      for (int e = 0; e < V; ++e) m.A[e] = fresh ? -1.f : m.A[e];
     }
-    lm_scan_group<V, true>(m, s_A, s_B, q.aggA, q.aggB, q.groupA, q.groupB, g, c, q.chunks, q.dim, col, lane, wv);
+    lm_scan_group<V, true>(m.map(fresh), s_W, s_B, q.aggW, q.aggB, q.groupW, q.groupB, g, c, q.chunks, q.dim, col, lane, wv);
   }
 }
 
 // the state (BACK: its gradient) that enters a chunk, from the one that enters its group
 template <class T, int V>
 __device__ __forceinline__ void lm_scan_enter(const LmScan<T>& q, u32 c, u32 col, float (&v)[V]) {
-  float a[V], b[V];
+  float w[V], b[V];
   lm_row_f32<V>(q.groupB, q.dim, c / kLmGroup, col, v);
-  lm_row_f32<V>(q.aggA, q.dim, c, col, a);
+  lm_row_f32<V>(q.aggW, q.dim, c, col, w);
   lm_row_f32<V>(q.aggB, q.dim, c, col, b);
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = a[e] < 0.f ? b[e] : __builtin_fmaf(a[e], v[e], b[e]);
+  for (int e = 0; e < V; ++e) v[e] = lm_map(w[e], v[e], b[e]);
 }
 
 // The states between the groups: groupB[c] becomes the state that enters group c (BACK: from behind).  A workgroup owns 16
@@ -390,8 +506,8 @@ __device__ __forceinline__ void lm_scan_enter(const LmScan<T>& q, u32 c, u32 col
 // 1 024 chunks of 1 024 columns, 17 us with 64 columns a workgroup and 16 threads each.
 constexpr u32 kLmCarryCols = 16, kLmCarryRuns = 64;
 template <bool BACK>
-__global__ void __launch_bounds__(kLmCarryCols * kLmCarryRuns) k_lm_scan_carry(const float* __restrict__ aggA, float* __restrict__ aggB, u32 chunks, u32 dim) {
-  __shared__ float s_A[kLmCarryRuns][kLmCarryCols], s_B[kLmCarryRuns][kLmCarryCols];
+__global__ void __launch_bounds__(kLmCarryCols * kLmCarryRuns) k_lm_scan_carry(const float* __restrict__ aggW, float* __restrict__ aggB, u32 chunks, u32 dim) {
+  __shared__ float s_W[kLmCarryRuns][kLmCarryCols], s_B[kLmCarryRuns][kLmCarryCols];
   const u32 cl = threadIdx.x % kLmCarryCols, run = threadIdx.x / kLmCarryCols;
   const u32 colBlocks = (dim + kLmCarryCols - 1) / kLmCarryCols;
   for (u32 block = blockIdx.x; block < colBlocks; block += gridDim.x) {
@@ -402,34 +518,34 @@ __global__ void __launch_bounds__(kLmCarryCols * kLmCarryRuns) k_lm_scan_carry(c
     auto at = [&](u32 c) { return (u64)(BACK ? chunks - 1 - c : c) * dim + col; };
     // up to kHold maps of a run stay in registers for the second walk
     constexpr u32 kHold = 16;
-    float a[kHold], b[kHold];
+    float w[kHold], b[kHold];
     auto load = [&](u32 c) {
 #pragma unroll
       for (u32 k = 0; k < kHold; ++k) {
         const u32 ck = c + k < c1 ? c + k : c1 - 1;
-        a[k] = aggA[at(ck)];
+        w[k] = aggW[at(ck)];
         b[k] = aggB[at(ck)];
       }
     };
-    float A = 1.f, B = 0.f;
+    float W = 0.f, B = 0.f;
     if (on) {
       for (u32 c = c0; c < c1; c += kHold) {
         load(c);
 #pragma unroll
         for (u32 k = 0; k < kHold; ++k) {
           if (c + k < c1) {
-            B = a[k] < 0.f ? b[k] : __builtin_fmaf(a[k], B, b[k]);
-            A = a[k] < 0.f || A < 0.f ? -1.f : A * a[k];
+            B = lm_map(w[k], B, b[k]);
+            W = lm_map_weight_then(W, w[k]);
           }
         }
       }
     }
-    s_A[run][cl] = A;
+    s_W[run][cl] = W;
     s_B[run][cl] = B;
     __syncthreads();
     float v = 0.f;   // (no state enters the first chunk: its sentences begin inside it)
 #pragma unroll 8
-    for (u32 w = 0; w < run; ++w) v = s_A[w][cl] < 0.f ? s_B[w][cl] : __builtin_fmaf(s_A[w][cl], v, s_B[w][cl]);
+    for (u32 r = 0; r < run; ++r) v = lm_map(s_W[r][cl], v, s_B[r][cl]);
     if (on) {
       for (u32 c = c0; c < c1; c += kHold) {
         if (per > kHold) load(c);
@@ -437,7 +553,7 @@ __global__ void __launch_bounds__(kLmCarryCols * kLmCarryRuns) k_lm_scan_carry(c
         for (u32 k = 0; k < kHold; ++k) {
           if (c + k < c1) {
             aggB[at(c + k)] = v;
-            v = a[k] < 0.f ? b[k] : __builtin_fmaf(a[k], v, b[k]);
+            v = lm_map(w[k], v, b[k]);
           }
         }
       }

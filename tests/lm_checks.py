@@ -839,6 +839,92 @@ def large(E, dtype):
     assert rel(loss, want) <= 16 * R.U and rel(dh, wdh) <= torch.finfo(dtype).eps / 2 + 16 * R.U and rel(dtable, wdt) <= 300 * R.U
 
 
+# ---- long memories, infinities, padded batches -----------------------------------------------------------
+@check(dtype=[F32, BF16, F16], max_len=[0, 1])
+def scan_open_gates_do_not_drift(E, dtype, max_len):
+    """gates near one over a long sentence: the state is a mean over 1 / (1 - a) rows, so weights of state and input that do not
+    sum to one would show that many times over.  What 32-bit states cannot do without is the rounding of every row's result.
+    Those of N rows within the state's memory, N <= 1 / (2 (1 - a)), are off by at most U of it and independent (the rows
+    differ), so their sum has a standard deviation of at most U sqrt(N / 3) of the largest state; four roundings a row (the
+    result's, the map's of a chunk, the sum's and the step's of the gradient) double that, and six deviations are 7 U sqrt(N).
+    The weights' own roundings act on differences from the mean, without the factor: 20 U."""
+    rows = 20000
+    g = rng(17)
+    columns = [7.25, 8.0, 9.0, 10.0, 11.0, 3.0, 0.0, -9.0]
+    gate = torch.tensor(columns + [9.0, 9.0]).repeat(rows, 1)
+    gate[:, -2:] += torch.randn(rows, 2, generator=g)
+    gate = gate.to(dtype)
+    x, dh = (normal(g, rows, len(columns) + 2, dtype=dtype, mean=1.0, std=0.3) for _ in range(2))
+    state, dlast = torch.full((1, x.shape[1]), 0.25), torch.full((1, x.shape[1]), -3.0)
+    off = torch.tensor([0, rows], dtype=torch.int32)
+    # 64 bits
+    z, xd, dhd = gate.double(), x.double(), dh.double()
+    a, b = torch.sigmoid(z), torch.sigmoid(-z)
+    before, h, delta = torch.empty_like(xd), torch.empty_like(xd), torch.empty_like(xd)
+    v = state[0].double()
+    for t in range(rows):
+        before[t] = v
+        v = v + b[t] * (xd[t] - v)
+        h[t] = v
+    back = dlast[0].double()
+    for t in reversed(range(rows)):
+        delta[t] = dhd[t] + back
+        back = delta[t] * a[t]
+    memory = (0.5 / b.mean(0)).clamp(1, rows)
+    tol = (7 * memory.sqrt() + 20) * R.U
+    most, most_d = before.abs().amax(0).maximum(xd.abs().amax(0)), delta.abs().amax(0)
+    e_h, e_d = tol * most, tol * most_d
+    diff = (before - xd).abs()
+    want = [R.out_round(h, e_h.expand_as(h), dtype), R.out_round(v[None], e_h[None], F32),
+            R.out_round(delta * a * b * (before - xd), a * b * (e_d * diff + delta.abs() * e_h + 20 * R.U * delta.abs() * most), dtype),
+            R.out_round(delta * b, b * (e_d + 20 * R.U * delta.abs()), dtype), R.out_round(back[None], e_d[None], F32)]
+    od = E.to(off)
+    hg, last, saved = lm.scan(E.to(gate), E.to(x), od, E.to(state), max_len=max_len, save=True, **E.kw)
+    got = (hg, last) + lm.scan_grad(E.to(gate), E.to(x), E.to(dh), saved, od, E.to(state), E.to(dlast), max_len=max_len, **E.kw)
+    for what, p, q in zip(('h', 'last', 'dgate', 'dx', 'dstate'), got, want):
+        near(what, p, q)
+
+
+@check(dtype=[F32, BF16], max_len=[0, 1])
+def scan_infinite_inputs(E, dtype, max_len):
+    """an infinity is what the formula makes of it, in the columns that have it and in no other: infinite states behind an infinite
+    input, NaN where opposite ones meet; and differences beyond the largest number are no infinities"""
+    inf = float('inf')
+    rows, dim = 300, 70
+    g = rng(23)
+    gate, x, dh = normal(g, rows, dim, mean=1.0, dtype=dtype), normal(g, rows, dim, dtype=dtype), normal(g, rows, dim, dtype=dtype)
+    state, dlast = normal(g, 1, dim), normal(g, 1, dim)
+    od = torch.tensor([0, rows], dtype=torch.int32)
+
+    def run(gate, x, dh, state, dlast):
+        h, last, saved = lm.scan(E.to(gate), E.to(x), E.to(od), E.to(state), max_len=max_len, save=True, **E.kw)
+        return [t.cpu() for t in (h, last) + lm.scan_grad(E.to(gate), E.to(x), E.to(dh), saved, E.to(od), E.to(state), E.to(dlast), max_len=max_len, **E.kw)]
+
+    plain = run(gate, x, dh, state, dlast)
+    x[40, 3], x[41, 4], x[203, 4], state[0, 69], dh[250, 5], dlast[0, 6], dh[17, 8], dh[16, 8] = inf, inf, -inf, -inf, inf, -inf, inf, -inf
+    big = 3e38
+    x[60, 7], x[61, 7], gate[60, 7], gate[61, 7] = big, -big, 0, 0
+    gate[:, 9], state[0, 9], dlast[0, 9] = -9, inf, inf   # (their product over a chunk is below the smallest number)
+    dirty = [3, 4, 5, 6, 7, 8, 9, 69]
+    got = run(gate, x, dh, state, dlast)
+    clean = torch.ones(dim, dtype=torch.bool)
+    clean[dirty] = False
+    for what, a, b in zip(('h', 'last', 'dgate', 'dx', 'dstate'), got, plain):
+        equal(what + ' of the other columns', a[:, clean], b[:, clean])
+    h, last, dgate, dx, dstate = got
+    assert h[:40, 3].isfinite().all() and (h[40:, 3] == inf).all() and last[0, 3] == inf
+    assert (h[41:203, 4] == inf).all() and h[203:, 4].isnan().all() and last[0, 4].isnan()
+    assert (h[:, 69] == -inf).all() and last[0, 69] == -inf
+    assert (h[:, 9] == inf).all() and last[0, 9] == inf and (dx[:, 9] == inf).all() and dstate[0, 9] == inf
+    assert (dx[:251, 5] == inf).all() and dx[251:, 5].isfinite().all() and dstate[0, 5] == inf
+    assert (dx[:, 6] == -inf).all() and dstate[0, 6] == -inf
+    assert dx[18:, 8].isfinite().all() and dx[17, 8] == inf and dx[:17, 8].isnan().all() and dstate[0, 8].isnan()
+    # half of 3e38 and a half of the state, then a quarter of it and half of -3e38: rounded values of that size
+    want = torch.stack([x[60, 7].double() / 2, x[60, 7].double() / 4 + x[61, 7].double() / 2])
+    assert ((h[60:62, 7].double() - want).abs() <= torch.finfo(dtype).eps * 3e38).all()
+    assert h[:, 7].isfinite().all() and dx[:, 7].isfinite().all()
+
+
 def run_all(device, lib_path, path):
     E = Env(device, lib_path)
     results = {}
