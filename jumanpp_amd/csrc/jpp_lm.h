@@ -220,23 +220,20 @@ __device__ __forceinline__ void lm_gate(float z, float& a, float& b) {
 // A gate as the smaller of sigmoid(z) and sigmoid(-z), with the sign of z: a step's weights are it and what it leaves of one, so
 // they sum to one however they are rounded.  (Rounded apart, they miss it by up to 2^-24, and a state that is a mean over
 // 1 / (1 - a) rows shows that as many times over: 3e-4 of itself behind 40 000 gates of 10.)
-// A 16-bit row's outputs are rounded to 2^-12 or 2^-9, and the vector unit takes longer over a gate than memory over its element:
-// there without the corrections (exp within (3 + 1.3 |z|) 2^-24 of itself, the reciprocal within 2^-23).
-template <class T>
-__device__ __forceinline__ float lm_row_weight(float z) {
-  float e, r;
-  if constexpr (sizeof(typename T::store) == 4) {
-    e = lm_exp_neg(__builtin_fabsf(z));
-    r = lm_rcp(1.f + e);
-  } else {
-    e = lm_exp2(-__builtin_fabsf(z) * 1.44269504088896341f);
+// To full precision whatever the rows' type: their states, and the gradients of those, come back in 32 bits.  1 / (1 + 2^t (1 + lo
+// ln 2)), t the rounded y log2 e and lo what it misses: the instructions' 2 units of 2^-24 each, the rounding of 1 + lo ln 2 and of
+// the sum.  (t ends at 1000, where the weight is zero, so that an infinite y has no infinity taken from itself; a NaN comes
+// through lo.)
+__device__ __forceinline__ float lm_gate_weight(float z) {
+  constexpr float kL = 1.44269504088896341f, kLlo = 1.92596303e-8f, kLn2 = 0.693147180559945309f;
+  const float y = __builtin_fabsf(z), t = __builtin_fminf(y * kL, 1000.f);
+  const float lo = __builtin_fmaf(y, kLlo, __builtin_fmaf(y, kL, -t));
+  const float d = __builtin_fmaf(lm_exp2(t), __builtin_fmaf(lo, kLn2, 1.f), 1.f);
 #if defined(__HIP_DEVICE_COMPILE__)
-    r = __builtin_amdgcn_rcpf(1.f + e);
+  return __builtin_copysignf(__builtin_amdgcn_rcpf(d), z);
 #else
-    r = 1.f / (1.f + e);
+  return __builtin_copysignf(1.f / d, z);
 #endif
-  }
-  return __builtin_copysignf(e * r, z);
 }
 __device__ __forceinline__ bool lm_open(float w) { return (i32)LmF32::put(w) >= 0; }   // (a weight may be a zero with a sign)
 // a v + (1 - a) x, from the larger weight's side
@@ -274,7 +271,8 @@ __device__ __forceinline__ float lm_map(float w, float v, float B) {
   return w == kLmFresh ? B : r;
 }
 
-// sigmoid(z), as far as rows of T show it: for 16 bits within (5 + 1.3 |z|) 2^-24 of itself, for the reasons of lm_row_weight
+// sigmoid(z), as far as rows of T show it: their outputs are rounded to 2^-12 or 2^-9, so for 16 bits without the corrections of
+// lm_exp_neg and lm_rcp, within (5 + 1.3 |z|) 2^-24 of itself
 template <class T>
 __device__ __forceinline__ float lm_row_sigmoid(float z) {
   if constexpr (sizeof(typename T::store) == 4) {

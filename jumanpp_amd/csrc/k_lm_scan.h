@@ -111,7 +111,7 @@ __device__ __forceinline__ void lm_scan_rows_weights(const LmScan<T>& q, u32 r0,
     const LmPack<T, V> f = lm_load<T, V>(q.gate + (i64)r * q.gateStride + col), x = lm_load<T, V>(q.x + (i64)r * q.xStride + col);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float w = lm_row_weight<T>(f.get(e));
+      const float w = lm_gate_weight(f.get(e));
       const LmWeights p(w);
       v[e] = odd[e] ? __builtin_fmaf(p.a, v[e], p.b * x.get(e)) : lm_step(w, v[e], x.get(e));
     }
@@ -151,7 +151,7 @@ __device__ __forceinline__ void lm_scan_rows(const LmScan<T>& q, u32 r0, u32 r1,
     for (u32 i = 0; i < kLmSave; ++i) {
       if (i < cnt) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = lm_step(lm_row_weight<T>(f[i].get(e)), v[e], x[i].get(e));
+        for (int e = 0; e < V; ++e) v[e] = lm_step(lm_gate_weight(f[i].get(e)), v[e], x[i].get(e));
         lm_store<T, V, STREAM>(q.h + (i64)(t + i) * q.hStride + col, lm_pack<T, V>(v));
       }
     }
@@ -180,7 +180,7 @@ __device__ __forceinline__ void lm_scan_grad_rows_weights(const LmScan<T>& q, u3
     const LmPack<T, V> d = lm_load<T, V>(q.dh + (i64)r * q.dhStride + col);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float w = lm_row_weight<T>(f.get(k)), delta = d.get(k) + e[k], s = __builtin_fabsf(w);
+      const float w = lm_gate_weight(f.get(k)), delta = d.get(k) + e[k], s = __builtin_fabsf(w);
       const LmWeights p(w);
       dx[k] = odd[k] ? p.b * delta : lm_let_in(w, delta);
       e[k] = odd[k] ? p.a * delta : lm_kept(w, delta);
@@ -215,7 +215,7 @@ __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 senten
     for (u32 i = 0; i < kLmSave; ++i) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        w[i][k] = lm_row_weight<T>(f[i].get(k));
+        w[i][k] = lm_gate_weight(f[i].get(k));
         before[i][k] = v[k];
         v[k] = lm_step(w[i][k], v[k], x[i].get(k));
       }
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_agg(LmScan<T> q) {
           if (k < cnt) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              const float w = lm_row_weight<T>(f[k].get(e));
+              const float w = lm_gate_weight(f[k].get(e));
               m.pass(e, w);
               m.B[e] = lm_step(w, m.B[e], x[k].get(e));
             }
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
           if (k < cnt) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              const float w = lm_row_weight<T>(f[k].get(e));
+              const float w = lm_gate_weight(f[k].get(e));
               m.pass(e, w);
               m.B[e] = lm_kept(w, m.B[e] + d[k].get(e));
             }
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
             const LmPack<T, V> g = lm_load<T, V>(q.gate + (i64)r * q.gateStride + col), u = lm_load<T, V>(q.dh + (i64)r * q.dhStride + col);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              const float w = lm_row_weight<T>(g.get(e));
+              const float w = lm_gate_weight(g.get(e));
               B0[e] += u.get(e);
               B0[e] = odd[e] ? LmWeights(w).a * B0[e] : lm_kept(w, B0[e]);
             }

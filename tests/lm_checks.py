@@ -925,6 +925,26 @@ def scan_infinite_inputs(E, dtype, max_len):
     assert h[:, 7].isfinite().all() and dx[:, 7].isfinite().all()
 
 
+@check(dtype=[F32, BF16, F16])
+def scan_states_are_32_bit_states(E, dtype):
+    """what comes back in 32 bits is right to 32 bits, whatever the rows are: one step whose result is a gate's weight itself, whose
+    relative rounding is that of two instructions of 2 U each and two sums (6 U), and the step's (2 U)"""
+    z = torch.linspace(0.25, 80, 320).to(dtype).float()
+    n, dim = 4, len(z)
+    gate = torch.stack([-z, z, -z, z]).to(dtype)
+    x = torch.tensor([0.0, 1.0, 0.0, 1.0])[:, None].expand(n, dim).contiguous().to(dtype)
+    state = torch.tensor([1.0, 0.0, -3.0, 0.0])[:, None].expand(n, dim).contiguous()
+    dlast = torch.tensor([1.0, 0.0, 5.0, 0.0])[:, None].expand(n, dim).contiguous()
+    off = E.to(torch.arange(n + 1, dtype=torch.int32))
+    h, last, saved = lm.scan(E.to(gate), E.to(x), off, E.to(state), max_len=1, save=True, **E.kw)
+    _, _, dstate = lm.scan_grad(E.to(gate), E.to(x), torch.zeros_like(h), saved, off, E.to(state), E.to(dlast), max_len=1, **E.kw)
+    s = torch.sigmoid(-z.double())
+    scale = torch.tensor([1.0, 1.0, 3.0, 1.0], dtype=torch.float64)[:, None]
+    near('last', last, (torch.tensor([1.0, 1.0, -3.0, 1.0], dtype=torch.float64)[:, None] * s, R.SLACK * 8 * R.U * scale * s + R.TINY))
+    want = torch.stack([s, 0 * s, 5 * s, 0 * s])
+    near('dstate', dstate, (want, R.SLACK * 8 * R.U * want + R.TINY))
+
+
 def run_all(device, lib_path, path):
     E = Env(device, lib_path)
     results = {}
