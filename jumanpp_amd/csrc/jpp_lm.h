@@ -207,14 +207,11 @@ __device__ __forceinline__ float lm_exp_neg(float y) {
   return y > 104.f ? 0.f : __builtin_fmaf(e * lo, kLn2, e);
 }
 
-// a = sigmoid(z), b = 1 - a = sigmoid(-z), each to full relative precision: 1 - a would lose b's digits where the gate is
-// nearly open, and b is the weight of the input
-__device__ __forceinline__ void lm_gate(float z, float& a, float& b) {
+// to full relative precision at either end
+__device__ __forceinline__ float lm_sigmoid(float z) {
   const float e = lm_exp_neg(__builtin_fabsf(z));
-  const float r = lm_rcp(1.f + e), er = e * r;
-  const bool up = z >= 0.f;
-  a = up ? r : er;
-  b = up ? er : r;
+  const float r = lm_rcp(1.f + e);
+  return z >= 0.f ? r : e * r;
 }
 
 // A gate as the smaller of sigmoid(z) and sigmoid(-z), with the sign of z: a step's weights are it and what it leaves of one, so
@@ -271,24 +268,6 @@ __device__ __forceinline__ float lm_map(float w, float v, float B) {
   return w == kLmFresh ? B : r;
 }
 
-// sigmoid(z), as far as rows of T show it: their outputs are rounded to 2^-12 or 2^-9, so for 16 bits without the corrections of
-// lm_exp_neg and lm_rcp, within (5 + 1.3 |z|) 2^-24 of itself
-template <class T>
-__device__ __forceinline__ float lm_row_sigmoid(float z) {
-  if constexpr (sizeof(typename T::store) == 4) {
-    float a, b;
-    lm_gate(z, a, b);
-    return a;
-  } else {
-    const float d = 1.f + lm_exp2(z * -1.44269504088896341f);
-#if defined(__HIP_DEVICE_COMPILE__)
-    return __builtin_amdgcn_rcpf(d);
-#else
-    return 1.f / d;
-#endif
-  }
-}
-
 // softplus(z) = max(z, 0) + ln(1 + exp(-|z|)), s = sigmoid(z); ln(1 + e) with the rounding of 1 + e put back
 __device__ __forceinline__ float lm_softplus(float z, float& s) {
   const float e = lm_exp_neg(__builtin_fabsf(z));
@@ -332,6 +311,19 @@ __device__ __forceinline__ float lm_group_sum(float v) {
   if constexpr (N >= 32) v += wave_shfl_f32(v, lane_id() ^ 16);
   if constexpr (N >= 64) v += wave_shfl_f32(v, lane_id() ^ 32);
   return v;
+#endif
+}
+
+// Lane I of every aligned group of N lanes (N = 16 or 64), in all lanes of the group.
+template <int N, int I>
+__device__ __forceinline__ float lm_group_bcast(float v) {
+  static_assert((N == 16 || N == 64) && I < 16, "a row of lanes, or all of them");
+#if defined(JPP_EMU) || !defined(__HIP_DEVICE_COMPILE__)
+  return wave_shfl_f32(v, (lane_id() & ~(N - 1)) + I);
+#else
+  if constexpr (N == 64) return wave_bcast_f32(v, I);
+  const int x = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, 0x150 + I, 0xf, 0xf, false));   // row_newbcast
 #endif
 }
 

@@ -286,13 +286,12 @@ __global__ void __launch_bounds__(kLmThreads)
       const float biasL = q.constant + lnL;
       // (a candidate that names no word reads the target's row and leaves with a gradient of zero)
       const u64 atL = lm_address(table + (u64)(rowL < q.vocab ? rowL : target) * (u64)q.tableStride);
-      // lane k keeps what is candidate k's alone: its logit now, its loss and gradient once for all 64 behind the loop.  In
-      // the loop a group makes the gradient of its candidate only as far as dh needs it.
+      // lane k keeps what is candidate k's alone: its logit now, its loss and gradient once for all 64 behind the loop
       float zL = 0.f;
       // candidates k0 .. k0 + R kGroups - 1, those behind kn as ones without a word
       auto rows = [&](auto many, u32 k0) {
         constexpr u32 R = decltype(many)::value;
-        static_assert(R * kGroups < 64, "a step does not pass the 64th candidate");
+        static_assert(R * kGroups < 64 && R <= 8, "a step does not pass the 64th candidate");
         LmRowPart<T, V, G, NV, FULL> b[R];
         const S* row[R];
 #pragma unroll
@@ -303,6 +302,7 @@ __global__ void __launch_bounds__(kLmThreads)
         if (kb + k0 == 0) fetch_rest(t + step);
         constexpr u64 kThese = (u64{1} << (R * kGroups)) - 1;
         const bool all = ((named >> k0) & kThese) == kThese;
+        float zg = 0.f;   // of the group's candidate gl
 #pragma unroll
         for (u32 u = 0; u < R; ++u) {
           const u32 k1 = k0 + u * kGroups, k = k1 + grp;
@@ -317,16 +317,27 @@ __global__ void __launch_bounds__(kLmThreads)
           // (lane k of the 64 reads group k mod kGroups)
           const float mine = kGroups == 1 ? z : wave_shfl_f32(z, (int)(((u32)lane & (kGroups - 1)) * G));
           zL = (u32)lane - k1 < kGroups ? mine : zL;
-          if constexpr (DH && !BLOCKS) {
-            const float s = kb + k == 0 ? -1.f : 1.f;
-            float gk = lm_row_sigmoid<T>(s * z) * (s * w);
-            if (!all) {   // (a branch around the sum, on its candidates or on their number, has the compiler copy the sum: 16 moves a row)
-              const bool ok = ((named >> k) & 1u) != 0;
-              gk = ok ? gk : 0.f;
-              b[u].keep(ok);
+          if constexpr (DH && !BLOCKS) zg = gl == u ? z : zg;
+        }
+        if constexpr (DH && !BLOCKS) {
+          // a lane a candidate makes the gradient once, and hands it to its group
+          const u32 kL = k0 + gl * kGroups + grp;
+          const float s = kb + kL == 0 ? -1.f : 1.f;
+          const float gL = lm_sigmoid(s * zg) * (s * w);
+          auto add = [&](auto at) {
+            constexpr int I = decltype(at)::value;
+            if constexpr (I < (int)R) {
+              float gk = lm_group_bcast<G, I>(gL);
+              if (!all) {   // (a branch around the sum, on its candidates or on their number, has the compiler copy the sum: 16 moves a row)
+                const bool ok = ((named >> (k0 + (u32)I * kGroups + grp)) & 1u) != 0;
+                gk = ok ? gk : 0.f;
+                b[I].keep(ok);
+              }
+              acc.template add<T, G>(gk, b[I]);
             }
-            acc.template add<T, G>(gk, b[u]);
-          }
+          };
+          add(LmConst<0>()), add(LmConst<1>()), add(LmConst<2>()), add(LmConst<3>());
+          add(LmConst<4>()), add(LmConst<5>()), add(LmConst<6>()), add(LmConst<7>());
         }
       };
       u32 k0 = 0;

@@ -945,6 +945,35 @@ def scan_states_are_32_bit_states(E, dtype):
     near('dstate', dstate, (want, R.SLACK * 8 * R.U * want + R.TINY))
 
 
+@check(dtype=[F32, BF16, F16], dim=[8, 128, 600])
+def nce_dh_is_summed_in_32_bits(E, dtype, dim):
+    """far scores whose parts of dh nearly cancel: what is left shows the precision of each part, which is rounded to the type only
+    in the end.  A part's gradient is within 7 U (sigmoid 6 U, weight), the sum of three parts within 5 U of their magnitudes."""
+    pairs = [(-20.0, -19.5), (-40.0, -39.0), (-60.0, -58.5), (-12.0, -11.75), (8.0, -7.5), (30.0, 25.0), (-3.0, -2.5), (-80.0, -78.0)]
+    n, cands = len(pairs), 3
+    h = torch.zeros(n, dim)
+    h[:, 0] = 1
+    table = torch.zeros(2 * n + 1, dim, dtype=torch.float64)
+    table[2 * n, 0] = 1.0
+    g = rng(31)
+    for i, (z1, z2) in enumerate(pairs):
+        table[2 * i, 0], table[2 * i + 1, 0] = z1, z2
+        w = (torch.rand(dim - 1, generator=g) + 1).to(dtype).double()
+        ratio = torch.sigmoid(torch.tensor(z1, dtype=torch.float64)) / torch.sigmoid(torch.tensor(z2, dtype=torch.float64))
+        table[2 * i, 1:], table[2 * i + 1, 1:] = w, -(w * ratio)
+    table = table.to(dtype)
+    ids = torch.stack([torch.full((n,), 2 * n), torch.arange(n) * 2, torch.arange(n) * 2 + 1], 1).to(torch.int32)
+    _, dh, _ = lm.nce_loss(E.to(h.to(dtype)), E.to(table), E.to(ids), E.to(torch.zeros(2 * n + 1)), 0.0, **E.kw)
+    rows = table.double()[ids.long()]
+    z = rows[:, :, 0]   # (exact: products with one and zero)
+    gz = torch.sigmoid(z)
+    gz[:, 0] = -torch.sigmoid(-z[:, 0])
+    parts = gz[:, :, None] * rows
+    want = parts.sum(1)
+    assert (want.abs()[:, 1:] < 0.01 * parts.abs().sum(1)[:, 1:]).any()
+    near('dh', dh, R.out_round(want, 12 * R.U * parts.abs().sum(1), dtype))
+
+
 def run_all(device, lib_path, path):
     E = Env(device, lib_path)
     results = {}
