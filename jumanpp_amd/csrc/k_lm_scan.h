@@ -590,21 +590,23 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_chunk(LmScan<T> q) {
     const u32 pack = cb * 64u + (u32)lane;
     const u32 col = lm_col<V>(pack < packs ? pack : packs - 1, q.dim);
     const u32 r0 = c * q.chunk, r1 = q.rows - r0 < q.chunk ? q.rows : r0 + q.chunk;
-    u32 i = uni(lm_sentence_of(q.offsets, q.n, r0, lane));
-    if (i == q.n) i = 0;   // the batch begins behind r0
-    for (u32 t = r0; i < q.n; ++i) {
-      const u32 begin = lm_offset(q.offsets, i, q.rows), end = lm_offset(q.offsets, i + 1, q.rows);
-      if (begin >= r1) break;
-      if (end <= t || end <= begin) continue;
+    const u32 first = lm_offset(q.offsets, 0, q.rows);
+    u32 t = first > r0 ? first : r0;
+    if (t >= r1) continue;   // the batch begins behind the chunk
+    // From sentence to sentence; sentences without a row may be many, so they are passed over by a search.
+    for (u32 i = uni(lm_sentence_of(q.offsets, q.n, t, lane)); i < q.n;) {
+      const u32 begin = lm_offset(q.offsets, i, q.rows), end = lm_offset(q.offsets, i + 1, q.rows), to = end < r1 ? end : r1;
       if (begin > t) t = begin;
+      if (t >= to) break;   // (behind the last sentence)
       float v[V];
       if (begin >= r0) lm_row_f32<V>(q.state, q.stateStride, i, col, v);
       else lm_scan_enter<T, V>(q, c, col, v);
-      const u32 to = end < r1 ? end : r1;
       lm_scan_rows<T, V, SAVE, STREAM>(q, t, to, col, v);
       if (to == end && q.last != nullptr) lm_put_f32<V>(q.last, q.lastStride, i, col, v);
       t = to;
-      if (t == r1) break;
+      if (t == r1 || i + 1 == q.n) break;
+      ++i;
+      if (lm_offset(q.offsets, i + 1, q.rows) <= t) i = uni(lm_sentence_of(q.offsets, q.n, t, lane));
     }
   }
   lm_scan_empty<V>(q.offsets, q.n, q.rows, q.dim, q.colBlocks, q.state, q.stateStride, q.last, q.lastStride);
@@ -620,22 +622,23 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_chunk(LmScan<T> q) 
     const u32 pack = cb * 64u + (u32)lane;
     const u32 col = lm_col<V>(pack < packs ? pack : packs - 1, q.dim);
     const u32 r0 = c * q.chunk, r1 = q.rows - r0 < q.chunk ? q.rows : r0 + q.chunk;
-    // sentences from the one with the last row down to the one with the first
-    u32 i = uni(lm_sentence_of(q.offsets, q.n, r1 - 1, lane));
-    if (i == q.n) continue;   // the batch begins behind the chunk
-    for (u32 t = r1;; --i) {
+    // sentences from the one with the last row down to the one with the first, those without a row passed over
+    const u32 total = lm_offset(q.offsets, q.n, q.rows);
+    u32 t = total < r1 ? total : r1;
+    if (t <= r0) continue;   // the batch ends in front of the chunk
+    for (u32 i = uni(lm_sentence_of(q.offsets, q.n, t - 1, lane)); i < q.n;) {
       const u32 begin = lm_offset(q.offsets, i, q.rows), end = lm_offset(q.offsets, i + 1, q.rows);
-      if (end <= r0 && begin < end) break;
       const u32 to = end < t ? end : t, from = begin > r0 ? begin : r0;
-      if (from < to) {
-        float e[V];
-        if (end <= r1) lm_row_f32<V>(q.dlast, q.dlastStride, i, col, e);
-        else lm_scan_enter<T, V>(q, c, col, e);
-        lm_scan_grad_rows<T, V, STREAM>(q, i, begin, from, to, col, e);
-        if (from == begin && q.dstate != nullptr) lm_put_f32<V>(q.dstate, q.dstateStride, i, col, e);
-        t = from;
-      }
-      if (i == 0 || t == r0) break;
+      if (from >= to) break;   // (in front of the first sentence)
+      float e[V];
+      if (end <= r1) lm_row_f32<V>(q.dlast, q.dlastStride, i, col, e);
+      else lm_scan_enter<T, V>(q, c, col, e);
+      lm_scan_grad_rows<T, V, STREAM>(q, i, begin, from, to, col, e);
+      if (from == begin && q.dstate != nullptr) lm_put_f32<V>(q.dstate, q.dstateStride, i, col, e);
+      t = from;
+      if (t == r0 || i == 0) break;
+      --i;
+      if (lm_offset(q.offsets, i, q.rows) >= t) i = uni(lm_sentence_of(q.offsets, q.n, t - 1, lane));
     }
   }
   lm_scan_empty<V>(q.offsets, q.n, q.rows, q.dim, q.colBlocks, q.dlast, q.dlastStride, q.dstate, q.dstateStride);

@@ -974,6 +974,56 @@ def nce_dh_is_summed_in_32_bits(E, dtype, dim):
     near('dh', dh, R.out_round(want, 12 * R.U * parts.abs().sum(1), dtype))
 
 
+# lengths, rows in front, rows behind: empty sentences at the ends and between, many more than rows
+EMPTY_CASES = (([1000] + [0] * 4000, 0, 984), ([0] * 3000 + [400, 0, 0, 300] + [0] * 3000 + [5, 270] + [0] * 70, 33, 700), ([0] * 2000, 0, 600),
+               ([0] * 2000, 600, 0), ([300] + [0, 1] * 200 + [0] * 64 + [290], 7, 9))
+
+
+@check(case=range(len(EMPTY_CASES)), dtype=[F32, F16])
+def scan_many_empty_sentences(E, case, dtype):
+    """a batch of a fixed number of sentences and rows, most of them unused: the rows and states of the others, and the states of
+    the empty ones"""
+    dim = 9
+    lengths, front, back = EMPTY_CASES[case]
+    offsets, rows, gate, x, dh, state, dlast, fill = scan_inputs((lengths, front, back), dim, dtype, case)
+    fill = fill.to(dtype).float()
+    want_h, want_last, _ = R.scan(gate, x, offsets, state, dtype, fill)
+    want = R.scan_grad(gate, x, offsets, state, dh, dlast, dtype, fill)
+    gd, xd, dhd, sd, ld, od = (E.to(t) for t in (gate, x, dh, state, dlast, offsets))
+    for max_len in (0, 1000, 1):
+        h, last, saved = raw_scan(E, gd, xd, od, sd, max_len, fill)
+        near('h', h, want_h)
+        near('last', last, want_last)
+        for what, a, b in zip(('dgate', 'dx', 'dstate'), raw_scan_grad(E, gd, xd, od, sd, max_len, saved, dhd, ld, fill), want):
+            near(what, a, b)
+
+
+@check(where_from=['behind', 'between'])
+def scan_empty_sentences_are_not_walked(E, where_from):
+    """what a batch's sentences without a row cost does not depend on whose way they lie in: as many in front of all rows, where no
+    chunk meets them, take as long.  (Walked one by one, those behind took ten times as long on the emulator.)"""
+    import time
+    n, rows, dim = 40000, 1984, 4
+    g = rng(1)
+    gate, x, dh = (E.to(normal(g, rows, dim)) for _ in range(3))
+
+    def took(lengths):
+        offsets = E.to(batch(lengths)[0])
+        best = 1e9
+        for _ in range(3):
+            t = time.perf_counter()
+            h, last, saved = lm.scan(gate, x, offsets, max_len=1000, save=True, **E.kw)
+            lm.scan_grad(gate, x, h, saved, offsets, max_len=1000, **E.kw)
+            if E.gpu:
+                torch.cuda.synchronize()
+            best = min(best, time.perf_counter() - t)
+        return best
+
+    none = [0] * n
+    plain = took(none + [700, 300])
+    assert took([700] + none + [300] if where_from == 'between' else [700, 300] + none) < 3 * plain
+
+
 def run_all(device, lib_path, path):
     E = Env(device, lib_path)
     results = {}
