@@ -19,7 +19,7 @@
  * A packed batch: `rows` rows and n + 1 int32 offsets, sentence i in rows offsets[i] .. offsets[i + 1] - 1 (none: an empty
  * sentence).  The offsets must not fall; they are on the device and are not checked (offsets that fall or leave
  * 0 .. rows give unspecified values in the outputs' own rows, never an access outside them).  Rows before offsets[0] and
- * from offsets[n] on belong to no sentence: outputs leave them as they were.
+ * from offsets[n] on belong to no sentence: outputs leave them as they were, or clear them (JPPGPU_LM_CLEAR_REST).
  *
  * Return codes and messages: jppgpu.h (JPPGPU_OK, JPPGPU_INVALID_PARAMETER, ..., jppgpu_last_error).  A refused call has
  * enqueued nothing.
@@ -35,11 +35,13 @@ extern "C" {
 
 /* element types */
 enum { JPPGPU_LM_F32 = 0, JPPGPU_LM_BF16 = 1, JPPGPU_LM_F16 = 2 };
+/* or'ed to the type of a packed batch's result (h, dgate, dx): its rows that belong to no sentence are set to zero */
+enum { JPPGPU_LM_CLEAR_REST = 0x100 };
 
 typedef struct {
   void* data;       /* first element; may be NULL where the matrix has no rows, or where it is optional */
   int64_t stride;   /* elements from one row to the next */
-  int32_t type;     /* JPPGPU_LM_* */
+  int32_t type;     /* JPPGPU_LM_F32, _BF16 or _F16 */
   int32_t reserved; /* 0 */
 } jppgpu_lm_matrix;
 

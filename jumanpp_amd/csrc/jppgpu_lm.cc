@@ -98,15 +98,19 @@ constexpr int64_t kMaxIndex = 0x7fffffff;   // words, packed rows, sentences, en
 
 int bytes_of(int32_t type) { return type == JPPGPU_LM_F32 ? 4 : 2; }
 
-enum Need { kNeeded, kOptional };
+int32_t type_of(const jppgpu_lm_matrix* m) { return m->type & ~JPPGPU_LM_CLEAR_REST; }
+bool cleared(const jppgpu_lm_matrix* m) { return (m->type & JPPGPU_LM_CLEAR_REST) != 0; }
+
+enum Need { kNeeded, kOptional, kBatchResult };   // (kBatchResult: needed, and may have its other rows cleared)
 
 // nullptr, or what is wrong with the matrix
 const char* bad_matrix(const jppgpu_lm_matrix* m, int64_t rows, int64_t dim, Need need) {
   if (m == nullptr) return need == kOptional ? nullptr : "a matrix is missing";
   if (m->reserved != 0) return "jppgpu_lm_matrix::reserved is not 0";
-  if (m->type != JPPGPU_LM_F32 && m->type != JPPGPU_LM_BF16 && m->type != JPPGPU_LM_F16) return "unknown element type";
+  const int32_t type = need == kBatchResult ? type_of(m) : m->type;
+  if (type != JPPGPU_LM_F32 && type != JPPGPU_LM_BF16 && type != JPPGPU_LM_F16) return "unknown element type";
   if (m->data == nullptr) return need == kOptional || rows == 0 ? nullptr : "a matrix has no data";
-  if (reinterpret_cast<uintptr_t>(m->data) % (uintptr_t)bytes_of(m->type) != 0) return "a matrix does not start on an element";
+  if (reinterpret_cast<uintptr_t>(m->data) % (uintptr_t)bytes_of(type) != 0) return "a matrix does not start on an element";
   if (m->stride < dim || m->stride > kMaxStride) return "the stride of a matrix is shorter than its rows, or beyond 2^32 - 1";
   return nullptr;
 }
@@ -375,11 +379,19 @@ u32 scan_chunk(u64 rows, u64 n, u64 dim, u64 maxLen) {
   return (u32)(chunk < 32 ? 32 : chunk < (1u << 30) ? chunk : 1u << 30);
 }
 
+// Workgroups of a kernel that walks sentences: a wavefront each and column block, and where rows of no sentence are to be cleared,
+// of which the host does not know how many there are, one for 64 KB of all rows, up to four a compute unit.
+template <class T>
+u64 scan_blocks(const LmScan<T>& q) {
+  const u64 blocks = div_up((u64)q.n * q.colBlocks, kLmThreads / 64), rest = div_up((u64)q.rows * q.dim * sizeof(typename T::store), 1 << 16);
+  return q.clear == 0 || rest <= blocks ? blocks : blocks > 1024 ? blocks : rest < 1024 ? rest : 1024;
+}
+
 template <class T, int V, bool STREAM>
 void launch_scan(Launcher& go, const LmScan<T>& q) {
   const u64 waves = kLmThreads / 64;
   if (q.chunk == 0) {
-    const u64 blocks = div_up((u64)q.n * q.colBlocks, waves);
+    const u64 blocks = scan_blocks(q);
     if (q.saved != nullptr) go(k_lm_scan_seq<T, V, true, STREAM>, blocks, kLmThreads, q);
     else go(k_lm_scan_seq<T, V, false, STREAM>, blocks, kLmThreads, q);
     return;
@@ -395,7 +407,7 @@ template <class T, int V, bool STREAM>
 void launch_scan_grad(Launcher& go, const LmScan<T>& q) {
   const u64 waves = kLmThreads / 64;
   if (q.chunk == 0) {
-    go(k_lm_scan_grad_seq<T, V, STREAM>, div_up((u64)q.n * q.colBlocks, waves), kLmThreads, q);
+    go(k_lm_scan_grad_seq<T, V, STREAM>, scan_blocks(q), kLmThreads, q);
     return;
   }
   const u64 blocks = div_up((u64)q.chunks * q.colBlocks, waves), groups = div_up(q.chunks, kLmGroup) * q.colBlocks;
@@ -449,6 +461,7 @@ void run_scan(Launcher& go, const ScanArgs& s, bool grad) {
   }
   q.saved = s.saved;
   if (!grad) {
+    q.clear = cleared(s.h) ? kLmClearRows : 0;
     q.h = static_cast<S*>(s.h->data);
     q.hStride = s.h->stride;
     if (given(s.last)) {
@@ -456,6 +469,7 @@ void run_scan(Launcher& go, const ScanArgs& s, bool grad) {
       q.lastStride = s.last->stride;
     }
   } else {
+    q.clear = (cleared(s.dgate) ? kLmClearDgate : 0) | (cleared(s.dx) ? kLmClearDx : 0);
     q.dh = static_cast<const S*>(s.dh->data);
     q.dhStride = s.dh->stride;
     q.dgate = static_cast<S*>(s.dgate->data);
@@ -473,7 +487,7 @@ void run_scan(Launcher& go, const ScanArgs& s, bool grad) {
   }
   const u32 v = scan_pack(q.dim, s.x->type, grad);
   q.colBlocks = (u32)div_up(div_up(q.dim, v), 64);
-  q.chunk = scan_chunk((u64)s.rows, (u64)s.n, (u64)s.dim, (u64)s.maxLen);
+  q.chunk = s.n == 0 ? 0 : scan_chunk((u64)s.rows, (u64)s.n, (u64)s.dim, (u64)s.maxLen);
   if (q.chunk != 0) {
     q.chunks = (u32)div_up(q.rows, q.chunk);
     Carver c{static_cast<char*>(s.workspace)};
@@ -664,10 +678,10 @@ extern "C" int jppgpu_lm_scan(const jppgpu_lm_matrix* gate, const jppgpu_lm_matr
   s.saved = saved;
   s.workspace = workspace;
   if (int rc = check_scan(s)) return rc;
-  JPP_LM_REFUSE_IF(bad_matrix(h, rows, dim, kNeeded));
+  JPP_LM_REFUSE_IF(bad_matrix(h, rows, dim, kBatchResult));
   JPP_LM_REFUSE_IF(bad_matrix(last, n, dim, kOptional));
   JPP_LM_REFUSE_IF(bad_f32(saved));
-  JPP_LM_CHECK(h->type == x->type, "h is of the type of x");
+  JPP_LM_CHECK(type_of(h) == x->type, "h is of the type of x");
   JPP_LM_CHECK(!given(last) || last->type == JPPGPU_LM_F32, "states are 32-bit");
   JPP_LM_CHECK(!same_start(h->data, {gate->data, x->data, given(state) ? state->data : nullptr}) &&
                    !same_start(given(last) ? last->data : nullptr, {gate->data, x->data, h->data, given(state) ? state->data : nullptr}),
@@ -675,7 +689,7 @@ extern "C" int jppgpu_lm_scan(const jppgpu_lm_matrix* gate, const jppgpu_lm_matr
   if (int rc = bad_workspace(workspace, workspace_bytes, scan_workspace(rows, n, dim, max_len))) return rc;
   DeviceScope scope(device);
   if (scope.rc() != JPPGPU_OK) return scope.rc();
-  if (n == 0) return JPPGPU_OK;
+  if (n == 0 && !cleared(h)) return JPPGPU_OK;
   Launcher go{static_cast<jpp_stream_t>(stream)};
   switch (x->type) {
     case JPPGPU_LM_F32: run_scan<LmF32>(go, s, false); break;
@@ -707,13 +721,13 @@ extern "C" int jppgpu_lm_scan_grad(const jppgpu_lm_matrix* gate, const jppgpu_lm
   s.workspace = workspace;
   if (int rc = check_scan(s)) return rc;
   JPP_LM_REFUSE_IF(bad_matrix(dh, rows, dim, kNeeded));
-  JPP_LM_REFUSE_IF(bad_matrix(dgate, rows, dim, kNeeded));
-  JPP_LM_REFUSE_IF(bad_matrix(dx, rows, dim, kNeeded));
+  JPP_LM_REFUSE_IF(bad_matrix(dgate, rows, dim, kBatchResult));
+  JPP_LM_REFUSE_IF(bad_matrix(dx, rows, dim, kBatchResult));
   JPP_LM_REFUSE_IF(bad_matrix(dlast, n, dim, kOptional));
   JPP_LM_REFUSE_IF(bad_matrix(dstate, n, dim, kOptional));
   JPP_LM_REFUSE_IF(bad_f32(saved));
   JPP_LM_CHECK(rows == 0 || saved != nullptr, "the saved states are missing");
-  JPP_LM_CHECK(dh->type == x->type && dgate->type == x->type && dx->type == x->type, "the gradients of rows are of the type of x");
+  JPP_LM_CHECK(dh->type == x->type && type_of(dgate) == x->type && type_of(dx) == x->type, "the gradients of rows are of the type of x");
   JPP_LM_CHECK((!given(dlast) || dlast->type == JPPGPU_LM_F32) && (!given(dstate) || dstate->type == JPPGPU_LM_F32),
                "the gradients of states are 32-bit");
   const void* st = given(state) ? state->data : nullptr;
@@ -725,7 +739,7 @@ extern "C" int jppgpu_lm_scan_grad(const jppgpu_lm_matrix* gate, const jppgpu_lm
   if (int rc = bad_workspace(workspace, workspace_bytes, scan_workspace(rows, n, dim, max_len))) return rc;
   DeviceScope scope(device);
   if (scope.rc() != JPPGPU_OK) return scope.rc();
-  if (n == 0) return JPPGPU_OK;
+  if (n == 0 && !cleared(dgate) && !cleared(dx)) return JPPGPU_OK;
   Launcher go{static_cast<jpp_stream_t>(stream)};
   switch (x->type) {
     case JPPGPU_LM_F32: run_scan<LmF32>(go, s, true); break;

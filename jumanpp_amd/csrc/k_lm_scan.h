@@ -56,18 +56,18 @@ struct LmScan {
   i64 dgateStride, dxStride;
   float* dstate;          // or null
   i64 dstateStride;
+  u32 clear;              // kLmClear*: results whose rows of no sentence are set to zero
   // chunks
   u32 chunk, chunks;      // rows of a chunk (a multiple of kLmSave), chunks
   float *aggW, *aggB;     // [chunks][dim] map of the chunks of its group that lie in front of a chunk
   float *groupW, *groupB; // [groups][dim] map of a group of kLmGroup chunks; k_lm_scan_carry turns B into the state that enters it
 };
+enum { kLmClearRows = 1, kLmClearDgate = 1, kLmClearDx = 2 };
 constexpr u32 kLmGroup = kLmThreads / 64;   // chunks that a workgroup of the aggregating kernels takes, a wavefront each
 
 // the rows of sentence i, inside the batch whatever the offsets hold
-__device__ __forceinline__ u32 lm_offset(const i32* offsets, u32 i, u32 rows) {
-  const i32 o = as_global(offsets)[i];
-  return uni(o < 0 ? 0u : (u32)o < rows ? (u32)o : rows);
-}
+__device__ __forceinline__ u32 lm_inside(i32 o, u32 rows) { return uni(o < 0 ? 0u : (u32)o < rows ? (u32)o : rows); }
+__device__ __forceinline__ u32 lm_offset(const i32* offsets, u32 i, u32 rows) { return lm_inside(as_global(offsets)[i], rows); }
 
 // The last sentence that begins at or before `row`, or n where the batch begins behind it; 64 offsets a step, all lanes
 // taking part.  (Offsets that fall give some sentence, in as many steps.)
@@ -252,9 +252,39 @@ __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 senten
   }
 }
 
+// The rows in front of the first sentence and behind the last one, a wavefront per row and column block, over the grid.  The two
+// offsets are asked for when the kernel begins and looked at when the rest is done.
+struct LmRest {
+  i32 first, total;
+};
+template <class T>
+__device__ __forceinline__ LmRest lm_scan_rest(const LmScan<T>& q) {
+  LmRest r = {(i32)q.rows, (i32)q.rows};
+  if (q.clear != 0 && q.n != 0) {
+    r.first = as_global(q.offsets)[0];
+    r.total = as_global(q.offsets)[q.n];
+  }
+  return r;
+}
+template <class T, int V, bool STREAM>
+__device__ __forceinline__ void lm_scan_clear(const LmScan<T>& q, const LmRest& r, u32 which, typename T::store* out, i64 stride) {
+  if ((q.clear & which) == 0) return;
+  const u32 first = lm_inside(r.first, q.rows), total = lm_inside(r.total, q.rows);
+  const u64 tasks = ((u64)first + q.rows - total) * q.colBlocks;
+  for (u64 task = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6); task < tasks; task += (u64)gridDim.x * (kLmThreads / 64)) {
+    const u32 i = uni((u32)(task / q.colBlocks)), cb = uni((u32)(task - (u64)i * q.colBlocks));
+    const u32 pack = cb * 64u + (threadIdx.x & 63u);
+    if (pack * V >= q.dim) continue;
+    LmPack<T, V> zero;
+    zero.zero();
+    lm_store<T, V, STREAM>(out + (i64)(i < first ? i : total + (i - first)) * stride + lm_col<V>(pack, q.dim), zero);
+  }
+}
+
 // ---- a wavefront per sentence and column block -----------------------------------
 template <class T, int V, bool SAVE, bool STREAM>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_seq(LmScan<T> q) {
+  const LmRest rest = lm_scan_rest(q);
   const u64 tasks = (u64)q.n * q.colBlocks;
   for (u64 task = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6); task < tasks; task += (u64)gridDim.x * (kLmThreads / 64)) {
     const u32 i = uni((u32)(task / q.colBlocks)), cb = uni((u32)(task - (u64)i * q.colBlocks));
@@ -267,10 +297,12 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_seq(LmScan<T> q) {
     if (r0 < r1) lm_scan_rows<T, V, SAVE, STREAM>(q, r0, r1, col, v);
     if (q.last != nullptr) lm_put_f32<V>(q.last, q.lastStride, i, col, v);
   }
+  lm_scan_clear<T, V, STREAM>(q, rest, kLmClearRows, q.h, q.hStride);
 }
 
 template <class T, int V, bool STREAM>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_seq(LmScan<T> q) {
+  const LmRest rest = lm_scan_rest(q);
   const u64 tasks = (u64)q.n * q.colBlocks;
   for (u64 task = (u64)blockIdx.x * (kLmThreads / 64) + (threadIdx.x >> 6); task < tasks; task += (u64)gridDim.x * (kLmThreads / 64)) {
     const u32 i = uni((u32)(task / q.colBlocks)), cb = uni((u32)(task - (u64)i * q.colBlocks));
@@ -283,6 +315,8 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_seq(LmScan<T> q) {
     if (r0 < r1) lm_scan_grad_rows<T, V, STREAM>(q, i, r0, r0, r1, col, e);
     if (q.dstate != nullptr) lm_put_f32<V>(q.dstate, q.dstateStride, i, col, e);
   }
+  lm_scan_clear<T, V, STREAM>(q, rest, kLmClearDgate, q.dgate, q.dgateStride);
+  lm_scan_clear<T, V, STREAM>(q, rest, kLmClearDx, q.dx, q.dxStride);
 }
 
 // ---- chunks ------------------------------------------------------------------------
@@ -582,6 +616,7 @@ __device__ __forceinline__ void lm_scan_empty(const i32* offsets, u32 n, u32 row
 
 template <class T, int V, bool SAVE, bool STREAM>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_chunk(LmScan<T> q) {
+  const LmRest rest = lm_scan_rest(q);
   const int lane = (int)(threadIdx.x & 63);
   const u32 packs = (q.dim + V - 1) / V;
   const u64 tasks = (u64)q.chunks * q.colBlocks;
@@ -610,10 +645,12 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_chunk(LmScan<T> q) {
     }
   }
   lm_scan_empty<V>(q.offsets, q.n, q.rows, q.dim, q.colBlocks, q.state, q.stateStride, q.last, q.lastStride);
+  lm_scan_clear<T, V, STREAM>(q, rest, kLmClearRows, q.h, q.hStride);
 }
 
 template <class T, int V, bool STREAM>
 __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_chunk(LmScan<T> q) {
+  const LmRest rest = lm_scan_rest(q);
   const int lane = (int)(threadIdx.x & 63);
   const u32 packs = (q.dim + V - 1) / V;
   const u64 tasks = (u64)q.chunks * q.colBlocks;
@@ -642,6 +679,8 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_chunk(LmScan<T> q) 
     }
   }
   lm_scan_empty<V>(q.offsets, q.n, q.rows, q.dim, q.colBlocks, q.dlast, q.dlastStride, q.dstate, q.dstateStride);
+  lm_scan_clear<T, V, STREAM>(q, rest, kLmClearDgate, q.dgate, q.dgateStride);
+  lm_scan_clear<T, V, STREAM>(q, rest, kLmClearDx, q.dx, q.dxStride);
 }
 
 }  // namespace jpp

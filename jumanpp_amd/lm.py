@@ -96,9 +96,12 @@ def _rows(t, what, n=None, dim=None):
     return _pack_matrix(t.data_ptr(), stride if rows > 1 else cols, code, 0)
 
 
-def _out(t, dim):
+_CLEAR_REST = 0x100   # JPPGPU_LM_CLEAR_REST
+
+
+def _out(t, dim, flags=0):
     """... of one of our own results"""
-    return _pack_matrix(t.data_ptr(), dim, _TYPES[t.dtype], 0)
+    return _pack_matrix(t.data_ptr(), dim, _TYPES[t.dtype] | flags, 0)
 
 
 def _ids(t, what='ids'):
@@ -174,7 +177,7 @@ def _batch(offsets, rows, device):
 def scan(gate, x, offsets=None, state=None, max_len=None, save=False, lib_path=None):
     """The gated linear recurrence h_t = a_t h_(t-1) + (1 - a_t) x_t, a = sigmoid(gate), over every sentence of a packed batch
     (offsets None: one sentence), from its row of `state` (float32 [n, dim]; None: zero).  Returns (h, last): h as x, last
-    float32 [n, dim] the states behind the sentences; rows of h that belong to no sentence are not written.  One row a
+    float32 [n, dim] the states behind the sentences; rows of h that belong to no sentence are zero.  One row a
     sentence is the serving step.  max_len: the longest sentence, where the host knows it; it decides how the work is split.
     save=True: (h, last, saved) with what scan_grad needs of the forward pass."""
     lib = _lib(lib_path)
@@ -189,14 +192,15 @@ def scan(gate, x, offsets=None, state=None, max_len=None, save=False, lib_path=N
     last = x.new_empty((n, dim), dtype=torch.float32)
     saved = x.new_empty((lib.jppgpu_lm_scan_saved(rows), dim), dtype=torch.float32) if save else None
     ws, wp, wn = _workspace(lib, 'jppgpu_lm_scan_workspace', (rows, n, dim, max_len), x)
-    _check(lib, lib.jppgpu_lm_scan(gv, xv, op, n, rows, dim, max_len, sv, _out(h, dim), _out(last, dim),
+    _check(lib, lib.jppgpu_lm_scan(gv, xv, op, n, rows, dim, max_len, sv, _out(h, dim, _CLEAR_REST), _out(last, dim),
                                    saved.data_ptr() if save else None, wp, wn, dev, stream))
     return (h, last, saved) if save else (h, last)
 
 
 def scan_grad(gate, x, dh, saved, offsets=None, state=None, dlast=None, max_len=None, lib_path=None):
     """The gradients (dgate, dx, dstate) of scan's inputs from those of its results, dh and dlast (float32; None: zero).
-    gate, x, offsets, state as in the scan(..., save=True) that returned `saved`."""
+    gate, x, offsets, state as in the scan(..., save=True) that returned `saved`.  Rows of dgate and dx that belong to no
+    sentence are zero."""
     lib = _lib(lib_path)
     dev, stream = _where(lib_path, x, gate, dh, saved, offsets, state, dlast)
     xv = _rows(x, 'x')
@@ -211,8 +215,8 @@ def scan_grad(gate, x, dh, saved, offsets=None, state=None, dlast=None, max_len=
     dgate, dx = x.new_empty((rows, dim)), x.new_empty((rows, dim))
     dstate = x.new_empty((n, dim), dtype=torch.float32)
     ws, wp, wn = _workspace(lib, 'jppgpu_lm_scan_workspace', (rows, n, dim, max_len), x)
-    _check(lib, lib.jppgpu_lm_scan_grad(gv, xv, op, n, rows, dim, max_len, sv, saved.data_ptr(), dv, lv, _out(dgate, dim),
-                                        _out(dx, dim), _out(dstate, dim), wp, wn, dev, stream))
+    _check(lib, lib.jppgpu_lm_scan_grad(gv, xv, op, n, rows, dim, max_len, sv, saved.data_ptr(), dv, lv, _out(dgate, dim, _CLEAR_REST),
+                                        _out(dx, dim, _CLEAR_REST), _out(dstate, dim), wp, wn, dev, stream))
     return dgate, dx, dstate
 
 

@@ -1024,6 +1024,52 @@ def scan_empty_sentences_are_not_walked(E, where_from):
     assert took([700] + none + [300] if where_from == 'between' else [700, 300] + none) < 3 * plain
 
 
+@check(case=[([5, 0, 7], 3, 9), ([300], 40, 70), ([0, 0], 0, 40), ([0], 30, 0), ([], 6, 7), ([9, 2], 0, 5000), ([2, 270, 1], 1000, 3000)], dtype=[F32, F16],
+       dim=[36, 130])
+def scan_rows_of_no_sentence_are_zero(E, case, dtype, dim):
+    """a padded batch: nothing is left in the results' other rows that a product with the whole matrix would take up"""
+    lengths, front, back = case
+    offsets, rows, gate, x, dh, state, dlast, _ = scan_inputs(case, dim, dtype, len(lengths))
+    gate[:front], x[:front], dh[:front] = (float('nan'),) * 3
+    gate[rows - back:], x[rows - back:], dh[rows - back:] = (float('nan'),) * 3
+    gd, xd, dhd, sd, ld, od = (E.to(t) for t in (gate, x, dh, state, dlast, offsets))
+    rest = torch.ones(rows, dtype=torch.bool)
+    rest[front:rows - back] = False
+    for max_len in (0, max(lengths + [1])):
+        fill = torch.full((rows, dim), float('nan'))
+        for _ in range(3):   # (memory that held something else)
+            soil = [E.to(torch.full((rows, dim), float('nan'), dtype=dtype)) for _ in range(4)]
+            del soil
+            h, last, saved = lm.scan(gd, xd, od, sd, max_len=max_len, save=True, **E.kw)
+            dgate, dx, dstate = lm.scan_grad(gd, xd, dhd, saved, od, sd, ld, max_len=max_len, **E.kw)
+            for what, t in zip(('h', 'dgate', 'dx'), (h, dgate, dx)):
+                assert (t.cpu()[rest] == 0).all(), what
+        # the caller's own matrices keep what they hold, unless they are to be cleared
+        left = raw_scan(E, gd, xd, od, sd, max_len, fill)
+        assert left[0].cpu()[rest].isnan().all()
+        equal('h', left[0].cpu()[~rest], h.cpu()[~rest])
+        equal('last', left[1], last)
+
+
+@check()
+def clearing_is_for_results_of_a_batch(E):
+    """the flag of a packed batch's results is no type of anything else"""
+    import struct
+    lib = lm._lib(E.lib_path)
+    a, b, c, out, out2, out3 = (torch.zeros(6, 8, device=E.device) for _ in range(6))
+    off = torch.tensor([0, 6], dtype=torch.int32, device=E.device)
+    st, last, saved, ids = torch.zeros(1, 8, device=E.device), torch.zeros(1, 8, device=E.device), torch.zeros(1, 8, device=E.device), off.new_zeros(6)
+    M = lambda t, clear=0: struct.pack('=QqiI', t.data_ptr(), 8, clear, 0)  # noqa: E731
+    dev, stream = lm._where(E.lib_path, a)
+    sc = lambda g=0, s=0, h=0, l=0: lib.jppgpu_lm_scan(M(a, g), M(b), off.data_ptr(), 1, 6, 8, 0, M(st, s), M(out, h), M(last, l),  # noqa: E731
+                                                       saved.data_ptr(), None, 0, dev, stream)
+    sg = lambda dh=0, dg=0, dx=0, ds=0: lib.jppgpu_lm_scan_grad(M(a), M(b), off.data_ptr(), 1, 6, 8, 0, M(st), saved.data_ptr(), M(c, dh), None,  # noqa: E731
+                                                                M(out2, dg), M(out3, dx), M(last, ds), None, 0, dev, stream)
+    em = lambda o=0: lib.jppgpu_lm_embed(M(a), 6, 8, struct.pack('=QiI', ids.data_ptr(), 4, 0), 6, 1.0, M(out, o), dev, stream)  # noqa: E731
+    assert sc() == sc(h=0x100) == sg() == sg(dg=0x100) == sg(dx=0x100) == sg(dg=0x100, dx=0x100) == em() == 0
+    assert 0 not in (sc(g=0x100), sc(s=0x100), sc(l=0x100), sc(h=0x200), sc(h=0x101), sg(dh=0x100), sg(ds=0x100), sg(dx=0x102), em(o=0x100))
+
+
 def run_all(device, lib_path, path):
     E = Env(device, lib_path)
     results = {}
