@@ -8,9 +8,10 @@ caller's own tensors, with their gradients, to train a model of one's own and to
     scores = nce_score(h, table, ids, constant)       loss, dh, dtable = nce_loss(h, table, ids, log_noise, constant, weight)
 
 Tensors live on one GPU; the work is enqueued on torch's current stream of that GPU, nothing waits, and every call may be
-captured into a graph.  Rows may have any stride, columns are contiguous; float32, bfloat16 and float16 (sums and states
-are 32-bit).  An id outside the vocabulary names no word: a row of zeros, no gradient, a score of -inf.  A packed batch is
-rows and n + 1 int32 offsets, as jppgpu_analyze_batch takes its sentences.
+captured into a graph.  They are no part of torch's record of a loss: gradients are the calls on the right, and a tensor that
+requires one is refused unless torch.no_grad() is on.  Rows may have any stride, columns are contiguous; float32, bfloat16 and
+float16 (sums and states are 32-bit).  An id outside the vocabulary names no word: a row of zeros, no gradient, a score of
+-inf.  A packed batch is rows and n + 1 int32 offsets, as jppgpu_analyze_batch takes its sentences.
 
 There is no CPU implementation behind this module.  (tests/ pass `lib_path` of the emulator build; test infrastructure.)
 """
@@ -66,8 +67,11 @@ def _refuse(why):
 
 
 def _where(lib_path, first, *others):
-    """(device ordinal, stream) of the call; every tensor on the device of the first"""
+    """(device ordinal, stream) of the call; every tensor on the device of the first, none that torch records gradients for"""
     index = first.get_device()
+    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in others)):
+        _refuse('a tensor requires a gradient, which these calls do not record: they have their own (embed_grad, scan_grad, '
+                'nce_loss); call them under torch.no_grad()')
     for t in others:
         if t is not None and t.get_device() != index:
             _refuse('the tensors are on different devices (%s, %s)' % (first.device, t.device))

@@ -1070,6 +1070,38 @@ def clearing_is_for_results_of_a_batch(E):
     assert 0 not in (sc(g=0x100), sc(s=0x100), sc(l=0x100), sc(h=0x200), sc(h=0x101), sg(dh=0x100), sg(ds=0x100), sg(dx=0x102), em(o=0x100))
 
 
+@check()
+def recorded_gradients_are_refused(E):
+    """no call is part of torch's graph of a loss: an input whose gradient is being recorded would lose it without a word"""
+    g = rng(41)
+    n, dim, vocab = 6, 12, 9
+    gate, x, table = E.to(normal(g, n, dim)), E.to(normal(g, n, dim)), E.to(normal(g, vocab, dim))
+    ids, cands = E.to(words(g, vocab, n)), E.to(words(g, vocab, n, 3))
+    off, state, ln, weight = E.to(torch.tensor([0, 2, n], dtype=torch.int32)), E.to(normal(g, 2, dim)), E.to(normal(g, vocab)), E.to(torch.rand(n, generator=g))
+    saved = lm.scan(gate, x, off, state, save=True, **E.kw)[2]
+    calls = [(lm.embed, [table, ids]), (lm.embed_grad, [x, ids, vocab]), (lm.scan, [gate, x, off, state]),
+             (lm.scan_grad, [gate, x, gate, saved, off, state, state]), (lm.nce_score, [x, table, cands, 0.5]),
+             (lm.nce_loss, [x, table, cands, ln, 0.5, weight])]
+    for fn, args in calls:
+        want = fn(*args, **E.kw)
+        for i, a in enumerate(args):
+            if not torch.is_tensor(a) or not a.is_floating_point():
+                continue
+            leaf = [a.detach().clone().requires_grad_() if j == i else b for j, b in enumerate(args)]
+            for these in (leaf, [b * 1 if torch.is_tensor(b) and b.requires_grad else b for b in leaf]):
+                try:
+                    fn(*these, **E.kw)
+                except JppGpuError as e:
+                    assert 'no_grad' in str(e), e
+                else:
+                    raise AssertionError('%s, argument %d: not refused' % (fn.__name__, i))
+                for off_ in (torch.no_grad, torch.inference_mode):
+                    with off_():
+                        got = fn(*these, **E.kw)
+                    for p, q in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+                        equal(fn.__name__, p, q)
+
+
 def run_all(device, lib_path, path):
     E = Env(device, lib_path)
     results = {}
