@@ -2,7 +2,9 @@
 it on the emulator build of the kernels, tests/test_lm_gpu.py in one child process on the GPU (torch has to load its HIP
 runtime before the library does, which the other GPU tests' process cannot promise):
 
-    python -u tests/lm_checks.py RESULTS.json
+    python -u tests/lm_checks.py [RESULTS.json]
+
+With a file, every check's result is in it and the status is that of the program; without one, the status says whether all passed.
 """
 import json
 import os
@@ -1102,7 +1104,7 @@ def recorded_gradients_are_refused(E):
                         equal(fn.__name__, p, q)
 
 
-def run_all(device, lib_path, path):
+def run_all(device, lib_path, path=None):
     E = Env(device, lib_path)
     results = {}
     for name, fn, where in CHECKS:
@@ -1116,15 +1118,22 @@ def run_all(device, lib_path, path):
         except Exception:
             results[name] = traceback.format_exc()
             print(results[name], flush=True)
-            if 'HIP error' in results[name] or 'hipError' in results[name]:
-                break   # (nothing more runs on a GPU that has failed)
-        with open(path, 'w') as f:
-            json.dump(results, f)
+        if path is not None:
+            with open(path, 'w') as f:
+                json.dump(results, f)
+        if 'HIP error' in results[name] or 'hipError' in results[name]:
+            break   # (nothing more runs on a GPU that has failed)
     return results
+
+
+def main(args, device='cuda'):
+    done = run_all(device, None, args[0] if args else None)
+    bad = [k for k, v in done.items() if v != 'ok']
+    due = sum(where != 'cpu' for _, _, where in CHECKS)
+    print('%s checks, %d failed' % (len(done) if len(done) == due else '%d of %d' % (len(done), due), len(bad)), flush=True)
+    return 1 if not args and (bad or len(done) < due) else 0
 
 
 if __name__ == '__main__':
     torch.zeros(1, device='cuda')   # torch's HIP runtime first
-    done = run_all('cuda', None, sys.argv[1])
-    bad = [k for k, v in done.items() if v != 'ok']
-    print('%d checks, %d failed' % (len(done), len(bad)), flush=True)
+    sys.exit(main(sys.argv[1:]))
