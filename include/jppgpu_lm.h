@@ -56,9 +56,10 @@ typedef struct {
 int jppgpu_lm_embed(const jppgpu_lm_matrix* table, int64_t vocab, int64_t dim, const jppgpu_lm_ids* ids, int64_t n, float scale,
                     const jppgpu_lm_matrix* out, int32_t device, void* stream);
 
-/* The gradient of the table: grad[v][:] = scale * sum over t with ids[t] = v of dy[t][:], the tokens summed in ascending
- * order by blocks whose size follows from (n, dim) alone; rows that no token names are zero.  grad: vocab x dim, 32-bit,
- * written whole.  dy: n x dim.  n < 2^31. */
+/* The gradient of the table: grad[v][:] = scale * sum over t with ids[t] = v of dy[t][:]; rows that no token names are zero.
+ * The tokens of a word are summed in ascending order in parts, and the parts in order; where a part ends follows from the sizes
+ * and from all ids, so the same inputs give the same bits, but other ids elsewhere may round a word's sum differently.
+ * grad: vocab x dim, 32-bit, written whole.  dy: n x dim.  n < 2^31. */
 int jppgpu_lm_embed_grad_workspace(int64_t n, int64_t vocab, int64_t dim, uint64_t* bytes);
 int jppgpu_lm_embed_grad(const jppgpu_lm_matrix* dy, const jppgpu_lm_ids* ids, int64_t n, int64_t vocab, int64_t dim, float scale,
                          const jppgpu_lm_matrix* grad, void* workspace, uint64_t workspace_bytes, int32_t device, void* stream);
