@@ -545,6 +545,10 @@ void launch_nce_row(Launcher& go, const LmNce& q, const void* h, const void* tab
   else launch_nce<T, G, NV, kLmPart>(go, q, h, table, ids, dh, loss);
 }
 
+// packs of 16 bytes of the longest row that a wavefront holds in registers; longer ones are walked in blocks
+constexpr u32 kNcePacks = 256;
+u32 nce_packs(u32 dim, i32 type) { return dim / (16 / (u32)bytes_of(type)); }
+
 template <class T>
 void run_nce(Launcher& go, const LmNce& q, const void* h, const void* table, LmIds ids, void* dh, bool loss) {
   const u32 packs = q.dim / (16 / (u32)sizeof(typename T::store));
@@ -552,7 +556,7 @@ void run_nce(Launcher& go, const LmNce& q, const void* h, const void* table, LmI
   else if (packs <= 32) launch_nce_row<T, 16, 2>(go, q, h, table, ids, dh, loss);
   else if (packs <= 64) launch_nce_row<T, 16, 4>(go, q, h, table, ids, dh, loss);
   else if (packs <= 128) launch_nce_row<T, 64, 2>(go, q, h, table, ids, dh, loss);
-  else if (packs <= 256) launch_nce_row<T, 64, 4>(go, q, h, table, ids, dh, loss);
+  else if (packs <= kNcePacks) launch_nce_row<T, 64, 4>(go, q, h, table, ids, dh, loss);
   else launch_nce<T, 64, 4, kLmBlocks>(go, q, h, table, ids, dh, loss);
 }
 
@@ -825,7 +829,11 @@ extern "C" int jppgpu_lm_nce_loss(const jppgpu_lm_matrix* h, const jppgpu_lm_mat
   q.out = loss;
   const u64 entries = (u64)n * (u64)cands;
   Carver c{static_cast<char*>(workspace)};
-  if (grads) q.g = c.take<float>(entries);
+  if (grads) {
+    // read by the sums by word, and for dh where rows are walked in blocks
+    float* g = c.take<float>(entries);
+    if (given(dtable) || nce_packs((u32)dim, h->type) > kNcePacks) q.g = g;
+  }
   dispatch_nce(go, q, h, table, ids_of(ids), const_cast<void*>(dhp), true);
   if (given(dtable) && vocab > 0) {
     SumPlan p(entries, (u64)vocab, (u64)dim, (u64)cands, true, h->type);

@@ -1104,6 +1104,25 @@ def recorded_gradients_are_refused(E):
                         equal(fn.__name__, p, q)
 
 
+@check(dim=[36, 300, 1500], dtype=[F32, BF16])
+def nce_dh_alone_leaves_the_workspace(E, dim, dtype):
+    """the gradients of the scores are written for the table's gradient alone (and for dh of rows that are walked in blocks)"""
+    n, k, vocab = 20, 7, 30
+    h, table, ids, used, log_noise, weight = nce_inputs(n, k, vocab, dim, dtype, 4)
+    h, table, ids, log_noise, weight = (E.to(t) for t in (h, table, ids, log_noise, weight))
+    _, want, _ = lm.nce_loss(h, table, ids, log_noise, 1.0, weight, **E.kw)
+    lib = lm._lib(E.lib_path)
+    dev, stream = lm._where(E.lib_path, h)
+    loss, dh = torch.empty(n, device=E.device), torch.empty_like(h)
+    ws, wp, wn = lm._workspace(lib, 'jppgpu_lm_nce_loss_workspace', (n, k, vocab, dim), h)
+    ws.fill_(255)
+    lm._check(lib, lib.jppgpu_lm_nce_loss(lm._rows(h, 'h'), lm._rows(table, 't'), vocab, dim, lm._ids(ids), n, k, log_noise.data_ptr(), 1.0,
+                                          weight.data_ptr(), loss.data_ptr(), lm._rows(dh, 'dh'), None, wp, wn, dev, stream))
+    equal('dh', dh, want)
+    in_blocks = dim * dh.element_size() // 16 > 256
+    assert in_blocks or bool((ws == 255).all())
+
+
 def run_all(device, lib_path, path=None):
     E = Env(device, lib_path)
     results = {}
