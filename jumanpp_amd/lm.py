@@ -69,12 +69,17 @@ def _refuse(why):
 def _where(lib_path, first, *others):
     """(device ordinal, stream) of the call; every tensor on the device of the first, none that torch records gradients for"""
     index = first.get_device()
-    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in others)):
+    recorded = torch.is_grad_enabled()
+    lost = recorded and first.requires_grad
+    for t in others:
+        if t is None:
+            continue
+        if t.get_device() != index:
+            _refuse('the tensors are on different devices (%s, %s)' % (first.device, t.device))
+        lost = lost or recorded and t.requires_grad
+    if lost:
         _refuse('a tensor requires a gradient, which these calls do not record: they have their own (embed_grad, scan_grad, '
                 'nce_loss); call them under torch.no_grad()')
-    for t in others:
-        if t is not None and t.get_device() != index:
-            _refuse('the tensors are on different devices (%s, %s)' % (first.device, t.device))
     if index < 0:
         if lib_path is None or first.device.type != 'cpu':
             _refuse('the tensors are on %s, not on a GPU' % first.device)
