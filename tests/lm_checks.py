@@ -1123,6 +1123,58 @@ def nce_dh_alone_leaves_the_workspace(E, dim, dtype):
     assert in_blocks or bool((ws == 255).all())
 
 
+@check('gpu', types=[(F32, BF16), (F32, F16), (F32, F32), (BF16, BF16), (F16, F16)], dim=[100, 257], size=['small', 'many', 'streamed'])
+def embed_many(E, types, dim, size):
+    """either side of where a thread takes four packs and of where results leave with the hint, at widths that no pack divides"""
+    per = 16 // torch.tensor([], dtype=types[1]).element_size()
+    packs = -(-dim // per)
+    four = 4 * 256 * 2048
+    n = {'small': (four - 1) // packs, 'many': -(-four // packs), 'streamed': (64 << 20) // (dim * torch.tensor([], dtype=types[1]).element_size()) + 1}[size]
+    vocab = 5003
+    table = torch.randn(vocab, dim, device='cuda').to(types[0])
+    ids = torch.randint(-3, vocab + 3, (n,), device='cuda', dtype=torch.int32)
+    got = lm.embed(table, ids, 0.7, dtype=types[1])
+    ok = (ids >= 0) & (ids < vocab)
+    scale = float(torch.tensor(0.7))
+    for part in torch.arange(n, device='cuda').split(50000):
+        exact = torch.where(ok[part][:, None], table[torch.where(ok, ids, 0)[part].long()].double() * scale, 0.0)
+        # the product rounded to 32 bits (U) and then to the type, or to the type at once: halves have an instruction for both
+        value, bound = R.out_round(exact, R.U * exact.abs(), types[1])
+        assert bool(((got[part].double() - value).abs() <= bound).all())
+
+
+@check('gpu', dtype=[F32, BF16, F16], dim=[130, 201, 300], long=[False, True])
+def scan_streamed(E, dtype, dim, long):
+    """results beyond where they leave with the hint, at widths whose last pack is moved back: a walk of short sentences, and chunks"""
+    rows = (64 << 20) // (dim * torch.tensor([], dtype=dtype).element_size()) + 77
+    g = rng(dim)
+    cut = torch.randint(0, rows + 1, (40 if long else rows // 20,), generator=g).sort().values
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), cut, torch.tensor([rows])]).to(torch.int32)
+    n = len(offsets) - 1
+    longest = int((offsets[1:] - offsets[:-1]).max())
+    d = torch.Generator(device='cuda')
+    d.manual_seed(dim)
+    gate, x, dh = (torch.randn(rows, dim, generator=d, device='cuda').mul_(2).add_(m).to(dtype) for m in (1.5, 0.0, 0.0))
+    state, dlast = (torch.randn(n, dim, generator=d, device='cuda') for _ in range(2))
+    od = offsets.cuda()
+    assert long or longest <= 256
+    h, last, saved = lm.scan(gate, x, od, state, max_len=longest, save=True)
+    out = lm.scan_grad(gate, x, dh, saved, od, state, dlast, max_len=longest)
+    for i in [0, 1, n // 3, n // 2, n - 2, n - 1] + torch.randint(0, n, (20 if not long else 2,), generator=g).tolist():
+        a, b = int(offsets[i]), int(offsets[i + 1])
+        if b - a > 12000:
+            continue
+        rows_of = [t[a:b].cpu() for t in (gate, x, dh)]
+        states = [t[i:i + 1].cpu() for t in (state, dlast)]
+        fill = torch.zeros(b - a, dim)
+        want_h, want_last, _ = R.scan(rows_of[0], rows_of[1], [0, b - a], states[0], dtype, fill)
+        near('h of sentence %d' % i, h[a:b], want_h)
+        near('last of sentence %d' % i, last[i:i + 1], want_last)
+        want = R.scan_grad(rows_of[0], rows_of[1], [0, b - a], states[0], rows_of[2], states[1], dtype, fill)
+        for what, p, q in zip(('dgate', 'dx', 'dstate'), (out[0][a:b], out[1][a:b], out[2][i:i + 1]), want):
+            near('%s of sentence %d' % (what, i), p, q)
+
+
 def run_all(device, lib_path, path=None):
     E = Env(device, lib_path)
     results = {}
