@@ -1175,6 +1175,89 @@ def scan_streamed(E, dtype, dim, long):
             near('%s of sentence %d' % (what, i), p, q)
 
 
+@check()
+def scores_reach_the_lattice(E):
+    """a language model of one's own as a host scorer: at every boundary the states of the global beam's left words (looked up and put
+    through one step of the recurrence) score all words that may follow, and the scores, which are those of the same model in 64
+    bits, go into the analysis's cells and change its paths"""
+    import jumanpp_amd as J
+    import numpy as np
+    gold = os.path.join(ROOT, 'tests', 'golden')
+    lines = [l.rstrip('\n') for l in open(os.path.join(gold, 'mini.txt'), encoding='utf-8')]
+    vocab, dim, constant, unknown = 97, 32, 2.0, -4.0
+    g = rng(7)
+    gates, inputs, out = normal(g, vocab, dim), normal(g, vocab, dim, std=4.0), normal(g, vocab, dim)
+    dev = [E.to(t) for t in (gates, inputs, out)]
+
+    def word(node):
+        return int(node['eptr']) % vocab if node['eptr'] >= 0 else -1
+
+    def boundaries(lat):
+        """(first cell row, left words of the global beam, right words) of every scored boundary"""
+        for s in range(lat['n']):
+            if lat['status'][s] != 0 or int(lat['ncp'][s]) == 0:
+                continue
+            nb, bb = int(lat['node_base'][s]), int(lat['bnd_base'][s])
+            for b in range(bb + 2, bb + int(lat['ncp'][s]) + 3):
+                right = nb + int(lat['bnd_first'][b])
+                n = int(lat['bnd_count'][b])
+                if n == 0:
+                    continue   # (nothing starts here: no global beam)
+                ends = nb + int(lat['end_first'][b])
+                left = [nb + int(lat['end_nodes'][ends + int(lat['gbeam_entries'][b][i]['left'])]) for i in range(int(lat['gbeam_count'][b]))]
+                if left:
+                    yield right, [word(lat['nodes'][i]) for i in left], [word(lat['nodes'][right + r]) for r in range(n)]
+
+    def own(lat, idx, cells):
+        todo = list(boundaries(lat))
+        most = max(len(r) for _, _, r in todo)
+        ids = torch.tensor([w for _, left, _ in todo for w in left], dtype=torch.int32)
+        cands = torch.tensor([right + [-1] * (most - len(right)) for _, left, right in todo for _ in left], dtype=torch.int32)
+        idd, off = E.to(ids), E.to(torch.arange(len(ids) + 1, dtype=torch.int32))
+        h, _ = lm.scan(lm.embed(dev[0], idd, **E.kw), lm.embed(dev[1], idd, **E.kw), off, max_len=1, **E.kw)
+        scores = lm.nce_score(h, dev[2], E.to(cands), constant, **E.kw).cpu().numpy()
+        scores = np.where(np.isfinite(scores), scores, np.float32(unknown))
+        row = 0
+        for first, left, right in todo:
+            cells[first:first + len(right), :len(left), idx] = scores[row:row + len(left), :len(right)].T
+            row += len(left)
+
+    def in64(lat, idx, cells):
+        a, b, c = (t.double().numpy() for t in (gates, inputs, out))
+        for first, left, right in boundaries(lat):
+            for i, l in enumerate(left):
+                h = b[l] / (1 + np.exp(a[l])) if l >= 0 else np.zeros(dim)
+                for r, w in enumerate(right):
+                    cells[first + r, i, idx] = c[w] @ h - constant if w >= 0 else unknown
+
+    def paths(scorer, weight):
+        kept = []
+
+        def keeping(lat, idx, cells):
+            scorer(lat, idx, cells)
+            kept.append(cells[:, :, idx].copy())
+        ctx = J.Context(os.path.join(gold, 'mini.img'), lib_path=E.lib_path, host_scorer_weights=[weight])
+        res = ctx.analyze_scored(lines, [keeping]).fetch(top1=True)
+        got = []
+        for s in range(len(lines)):
+            n = int(res.path_len[s]) if res.status[s] == 0 else 0
+            nodes = res.nodes[int(res.node_base[s]):int(res.node_base[s]) + n]
+            got.append([(int(x['eptr']), int(x['start']), int(x['end'])) for x in nodes])
+        return got, kept[0]
+
+    def replay(lat, idx, into):
+        into[:, :, idx] = cells
+
+    mine, cells = paths(own, 0.5)
+    _, cells64 = paths(in64, 0.5)
+    # 32-bit roundings of a state (10 U) and of a product of 32 terms (34 U) of magnitudes that sum to less than 100
+    assert np.abs(cells.astype(np.float64) - cells64).max() <= 50 * R.U * 100 and (cells64 != 0).sum() > 1000
+    # (two words unknown to the model score alike, so roundings may choose between paths: the paths are those of these scores)
+    assert mine == paths(replay, 0.5)[0]
+    without = paths(lambda lat, idx, cells: None, 0.5)[0]
+    assert sum(a != b for a, b in zip(mine, without)) >= 3, 'the scorer has to matter'
+
+
 def run_all(device, lib_path, path=None):
     E = Env(device, lib_path)
     results = {}
