@@ -235,9 +235,15 @@ __device__ __forceinline__ float lm_gate_weight(float z) {
 __device__ __forceinline__ bool lm_open(float w) { return (i32)LmF32::put(w) >= 0; }   // (a weight may be a zero with a sign)
 // a v + (1 - a) x, from the larger weight's side
 __device__ __forceinline__ float lm_step(float w, float v, float x) { return __builtin_fmaf(w, x - v, lm_open(w) ? v : x); }
-// a v and (1 - a) v
+// a v
 __device__ __forceinline__ float lm_kept(float w, float v) { return __builtin_fmaf(-w, v, lm_open(w) ? v : 0.f); }
-__device__ __forceinline__ float lm_let_in(float w, float v) { return __builtin_fmaf(w, v, lm_open(w) ? 0.f : v); }
+// a v, (1 - a) v, a (1 - a) v
+__device__ __forceinline__ void lm_parts(float w, float v, float& kept, float& in, float& both) {
+  const float s = __builtin_fabsf(w), p = s * v, q = __builtin_fmaf(-s, v, v);
+  kept = lm_open(w) ? q : p;
+  in = lm_open(w) ? p : q;
+  both = __builtin_fmaf(-s, p, p);
+}
 // The same from the two weights, for states that are not finite, or further than the largest number from what comes in: there
 // differences are NaN or infinite where the formula's value is not.
 struct LmWeights {
@@ -255,16 +261,18 @@ __device__ __forceinline__ bool lm_finite(float v) { return __builtin_fabsf(v) <
 // passes, also where v is no number.
 constexpr float kLmFresh = -2.f;
 __device__ __forceinline__ float lm_map_weight(float A, float C) { return C <= 0.5f ? C : -A; }   // C: 1 - A, made for itself
-// the map of weight w2 behind that of weight w1
-__device__ __forceinline__ float lm_map_weight_then(float w1, float w2) {
-  const float A1 = lm_open(w1) ? 1.f - w1 : -w1, C1 = lm_open(w1) ? w1 : 1.f + w1;
-  const float w = lm_map_weight(lm_kept(w2, A1), lm_step(w2, C1, 1.f));
-  return w1 == kLmFresh || w2 == kLmFresh ? kLmFresh : w;
-}
+// A v + B = whole v + (minus v + B), for finite v
+__device__ __forceinline__ float lm_map_whole(float w) { return lm_open(w) ? 1.f : 0.f; }
+__device__ __forceinline__ float lm_map_minus(float w) { return w == kLmFresh ? 0.f : -w; }
+// A v + B.  EXACT: also where v is not finite, or the difference v (A - 1) + B is not; a caller takes it where the other form's
+// result is not finite.  (A is never zero, though its product may be: an infinity passes.)
+template <bool EXACT>
 __device__ __forceinline__ float lm_map(float w, float v, float B) {
   float r = __builtin_fmaf(-w, v, B) + (lm_open(w) ? v : 0.f);
-  // (A is never zero, though its product may be: an infinity passes)
-  if (!lm_finite(r)) r = lm_finite(v) ? __builtin_fmaf(lm_open(w) ? 1.f - w : -w, v, B) : v + B;
+  if constexpr (EXACT) {
+    const float s = lm_finite(v) ? __builtin_fmaf(lm_open(w) ? 1.f - w : -w, v, B) : v + B;
+    r = lm_finite(r) ? r : s;
+  }
   return w == kLmFresh ? B : r;
 }
 

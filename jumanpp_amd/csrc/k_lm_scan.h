@@ -156,7 +156,7 @@ __device__ __forceinline__ void lm_scan_rows(const LmScan<T>& q, u32 r0, u32 r1,
       }
     }
     bool odd[V];
-    if (lm_odd<V>(v, odd)) {
+    if (__builtin_expect(lm_odd<V>(v, odd), 0)) {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] = v0[e];
       lm_scan_rows_weights<T, V, true, STREAM>(q, t, t + cnt, col, odd, v);
@@ -180,11 +180,16 @@ __device__ __forceinline__ void lm_scan_grad_rows_weights(const LmScan<T>& q, u3
     const LmPack<T, V> d = lm_load<T, V>(q.dh + (i64)r * q.dhStride + col);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float w = lm_gate_weight(f.get(k)), delta = d.get(k) + e[k], s = __builtin_fabsf(w);
+      const float w = lm_gate_weight(f.get(k)), delta = d.get(k) + e[k];
       const LmWeights p(w);
-      dx[k] = odd[k] ? p.b * delta : lm_let_in(w, delta);
-      e[k] = odd[k] ? p.a * delta : lm_kept(w, delta);
-      df[k] = delta * __builtin_fmaf(-s, s, s) * (v[k] - x.get(k));
+      float both;
+      lm_parts(w, delta, e[k], dx[k], both);
+      if (odd[k]) {
+        dx[k] = p.b * delta;
+        e[k] = p.a * delta;
+        both = p.a * p.b * delta;
+      }
+      df[k] = both * (v[k] - x.get(k));
     }
     lm_store<T, V, STREAM>(q.dgate + (i64)r * q.dgateStride + col, lm_pack<T, V>(df));
     lm_store<T, V, STREAM>(q.dx + (i64)r * q.dxStride + col, lm_pack<T, V>(dx));
@@ -229,10 +234,9 @@ __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 senten
         float df[V], dx[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float delta = d[i].get(k) + e[k], s = __builtin_fabsf(w[i][k]);
-          dx[k] = lm_let_in(w[i][k], delta);
-          e[k] = lm_kept(w[i][k], delta);
-          df[k] = delta * __builtin_fmaf(-s, s, s) * (before[i][k] - x[i].get(k));   // (a b = s (1 - s))
+          float both;
+          lm_parts(w[i][k], d[i].get(k) + e[k], e[k], dx[k], both);
+          df[k] = both * (before[i][k] - x[i].get(k));
         }
         lm_store<T, V, STREAM>(q.dgate + (i64)(t + i) * q.dgateStride + col, lm_pack<T, V>(df));
         lm_store<T, V, STREAM>(q.dx + (i64)(t + i) * q.dxStride + col, lm_pack<T, V>(dx));
@@ -240,7 +244,7 @@ __device__ __forceinline__ void lm_scan_grad_rows(const LmScan<T>& q, u32 senten
     }
     bool odd[V], oddV[V];
     const bool oddE = lm_odd<V>(e, odd);
-    if (lm_odd<V>(v, oddV) || oddE) {
+    if (__builtin_expect(lm_odd<V>(v, oddV) || oddE, 0)) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         odd[k] = odd[k] || oddV[k];
@@ -321,70 +325,70 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_seq(LmScan<T> q) {
 
 // ---- chunks ------------------------------------------------------------------------
 template <int V>
-struct LmMap {   // s -> A s + B; W: the weight of A (lm_map_weight)
-  float W[V], B[V];
-  __device__ __forceinline__ void one() {
-#pragma unroll
-    for (int e = 0; e < V; ++e) W[e] = B[e] = 0.f;
-  }
-  // this map, then the map (w, b)
-  __device__ __forceinline__ void then(int e, float w, float b) {
-    B[e] = lm_map(w, B[e], b);
-    W[e] = lm_map_weight_then(W[e], w);
-  }
-};
-// ... of rows, made row by row
-template <int V>
-struct LmRowsMap {
+struct LmMap {   // s -> A s + B
   float A[V], C[V], B[V];   // C = 1 - A
+  bool fresh;               // s -> B
   __device__ __forceinline__ void one() {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       A[e] = 1.f;
       C[e] = B[e] = 0.f;
     }
+    fresh = false;
   }
+  // the weight of this map, then of one of weight w
   __device__ __forceinline__ void pass(int e, float w) {
+    C[e] = __builtin_fmaf(w, A[e], lm_open(w) ? C[e] : 1.f);
     A[e] = lm_kept(w, A[e]);
-    C[e] = lm_step(w, C[e], 1.f);
   }
-  __device__ __forceinline__ LmMap<V> map(bool fresh) const {
-    LmMap<V> m;
+  // this map, then the map (w, b)
+  template <bool EXACT>
+  __device__ __forceinline__ void then(int e, float w, float b) {
+    pass(e, w);
+    B[e] = lm_map<EXACT>(w, B[e], b);
+    fresh = fresh || w == kLmFresh;   // (of one element, of all)
+  }
+  __device__ __forceinline__ float weight(int e) const { return fresh ? kLmFresh : lm_map_weight(A[e], C[e]); }
+  __device__ __forceinline__ void put(float* w, float* b, u32 dim, u32 row, u32 col) const {
+    float W[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      m.W[e] = fresh ? kLmFresh : lm_map_weight(A[e], C[e]);
-      m.B[e] = B[e];
-    }
-    return m;
+    for (int e = 0; e < V; ++e) W[e] = weight(e);
+    lm_put_f32<V>(w, dim, row, col, W);
+    lm_put_f32<V>(b, dim, row, col, B);
   }
 };
 
 // The maps of a workgroup's chunks, a wavefront each: what lies in front of a chunk inside the group, and the group's own.
 // BACK: in front is behind.
 template <int V, bool BACK>
-__device__ __forceinline__ void lm_scan_group(LmMap<V> m, float (&sW)[kLmGroup][64 * V], float (&sB)[kLmGroup][64 * V], float* aggW, float* aggB,
+__device__ __forceinline__ void lm_scan_group(const LmMap<V>& own, float (&sW)[kLmGroup][64 * V], float (&sB)[kLmGroup][64 * V], float* aggW, float* aggB,
                                               float* groupW, float* groupB, u32 group, u32 chunk, u32 chunks, u32 dim, u32 col, int lane, int wv) {
   // order of the walk
   const int at = BACK ? (int)kLmGroup - 1 - wv : wv;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    sW[at][lane * V + e] = m.W[e];
-    sB[at][lane * V + e] = m.B[e];
+    sW[at][lane * V + e] = own.weight(e);
+    sB[at][lane * V + e] = own.B[e];
   }
   __syncthreads();
-  m.one();
-  for (int w = 0; w < at; ++w)
+  LmMap<V> m;
+  auto front = [&](auto exact) {
+    bool finite = true;
+    m.one();
+    for (int w = 0; w < at; ++w)
 #pragma unroll
-    for (int e = 0; e < V; ++e) m.then(e, sW[w][lane * V + e], sB[w][lane * V + e]);
-  if (chunk < chunks) {
-    lm_put_f32<V>(aggW, dim, chunk, col, m.W);
-    lm_put_f32<V>(aggB, dim, chunk, col, m.B);
-  }
+      for (int e = 0; e < V; ++e) {
+        m.template then<decltype(exact)::value != 0>(e, sW[w][lane * V + e], sB[w][lane * V + e]);
+        finite = finite && lm_finite(m.B[e]);
+      }
+    return finite;
+  };
+  if (__builtin_expect(!front(LmConst<0>()), 0)) front(LmConst<1>());
+  if (chunk < chunks) m.put(aggW, aggB, dim, chunk, col);
   if (at == (int)kLmGroup - 1) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) m.then(e, sW[at][lane * V + e], sB[at][lane * V + e]);
-    lm_put_f32<V>(groupW, dim, group, col, m.W);
-    lm_put_f32<V>(groupB, dim, group, col, m.B);
+    for (int e = 0; e < V; ++e) m.template then<true>(e, sW[at][lane * V + e], sB[at][lane * V + e]);
+    m.put(groupW, groupB, dim, group, col);
   }
   __syncthreads();
 }
@@ -401,9 +405,8 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_agg(LmScan<T> q) {
     // (lanes behind the last column repeat it: the same loads, the same stores)
     const u32 pack = cb * 64u + (u32)lane;
     const u32 col = lm_col<V>(pack < packs ? pack : packs - 1, q.dim);
-    LmRowsMap<V> m;
+    LmMap<V> m;
     m.one();
-    bool fresh = false;   // nothing passes
     if (c < q.chunks) {
       const u32 r0 = c * q.chunk, r1 = q.rows - r0 < q.chunk ? q.rows : r0 + q.chunk;
       // only the sentence that holds the chunk's last row reaches past it
@@ -413,8 +416,8 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_agg(LmScan<T> q) {
         const u32 begin = lm_offset(q.offsets, i, q.rows), end = lm_offset(q.offsets, i + 1, q.rows);
         from = begin > r0 ? begin : r0;
         to = end < r1 ? end : r1;
-        fresh = begin >= r0;
-        if (fresh) lm_row_f32<V>(q.state, q.stateStride, i, col, m.B);
+        m.fresh = begin >= r0;
+        if (m.fresh) lm_row_f32<V>(q.state, q.stateStride, i, col, m.B);
       }
       for (u32 t = from; t < to; t += kLmSave) {
         const u32 cnt = to - t;
@@ -440,14 +443,14 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_agg(LmScan<T> q) {
           }
         }
         bool odd[V];
-        if (lm_odd<V>(m.B, odd)) {
+        if (__builtin_expect(lm_odd<V>(m.B, odd), 0)) {
 #pragma unroll
           for (int e = 0; e < V; ++e) m.B[e] = B0[e];
           lm_scan_rows_weights<T, V, false, false>(q, t, cnt < kLmSave ? to : t + kLmSave, col, odd, m.B);
         }
       }
     }
-    lm_scan_group<V, false>(m.map(fresh), s_W, s_B, q.aggW, q.aggB, q.groupW, q.groupB, g, c, q.chunks, q.dim, col, lane, wv);
+    lm_scan_group<V, false>(m, s_W, s_B, q.aggW, q.aggB, q.groupW, q.groupB, g, c, q.chunks, q.dim, col, lane, wv);
   }
 }
 
@@ -462,9 +465,8 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
     const u32 g = (u32)(block / q.colBlocks), cb = (u32)(block - (u64)g * q.colBlocks), c = g * kLmGroup + (u32)wv;
     const u32 pack = cb * 64u + (u32)lane;
     const u32 col = lm_col<V>(pack < packs ? pack : packs - 1, q.dim);
-    LmRowsMap<V> m;
+    LmMap<V> m;
     m.one();
-    bool fresh = false;   // nothing passes
     if (c < q.chunks) {
       const u32 r0 = c * q.chunk, r1 = q.rows - r0 < q.chunk ? q.rows : r0 + q.chunk;
       // only the sentence that holds the chunk's first row reaches in front of it
@@ -473,8 +475,8 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
       if (i < q.n) {
         const u32 end = lm_offset(q.offsets, i + 1, q.rows);
         to = end < r1 ? end : r1;
-        fresh = end <= r1;
-        if (fresh) lm_row_f32<V>(q.dlast, q.dlastStride, i, col, m.B);
+        m.fresh = end <= r1;
+        if (m.fresh) lm_row_f32<V>(q.dlast, q.dlastStride, i, col, m.B);
       }
       for (u32 end = to; end > r0;) {
         const u32 t = end - r0 > kLmSave ? end - kLmSave : r0;
@@ -502,7 +504,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
           }
         }
         bool odd[V];
-        if (lm_odd<V>(m.B, odd)) {
+        if (__builtin_expect(lm_odd<V>(m.B, odd), 0)) {
 #pragma unroll 1
           for (u32 r = end; r-- > t;) {
             const LmPack<T, V> g = lm_load<T, V>(q.gate + (i64)r * q.gateStride + col), u = lm_load<T, V>(q.dh + (i64)r * q.dhStride + col);
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_agg(LmScan<T> q) {
         end = t;
       }
     }
-    lm_scan_group<V, true>(m.map(fresh), s_W, s_B, q.aggW, q.aggB, q.groupW, q.groupB, g, c, q.chunks, q.dim, col, lane, wv);
+    lm_scan_group<V, true>(m, s_W, s_B, q.aggW, q.aggB, q.groupW, q.groupB, g, c, q.chunks, q.dim, col, lane, wv);
   }
 }
 
@@ -531,7 +533,7 @@ __device__ __forceinline__ void lm_scan_enter(const LmScan<T>& q, u32 c, u32 col
   lm_row_f32<V>(q.aggW, q.dim, c, col, w);
   lm_row_f32<V>(q.aggB, q.dim, c, col, b);
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = lm_map(w[e], v[e], b[e]);
+  for (int e = 0; e < V; ++e) v[e] = lm_map<true>(w[e], v[e], b[e]);
 }
 
 // The states between the groups: groupB[c] becomes the state that enters group c (BACK: from behind).  A workgroup owns 16
@@ -541,7 +543,7 @@ __device__ __forceinline__ void lm_scan_enter(const LmScan<T>& q, u32 c, u32 col
 constexpr u32 kLmCarryCols = 16, kLmCarryRuns = 64;
 template <bool BACK>
 __global__ void __launch_bounds__(kLmCarryCols * kLmCarryRuns) k_lm_scan_carry(const float* __restrict__ aggW, float* __restrict__ aggB, u32 chunks, u32 dim) {
-  __shared__ float s_W[kLmCarryRuns][kLmCarryCols], s_B[kLmCarryRuns][kLmCarryCols];
+  __shared__ float s_W[kLmCarryRuns][kLmCarryCols], s_B[kLmCarryRuns][kLmCarryCols], s_k[kLmCarryRuns][kLmCarryCols], s_m[kLmCarryRuns][kLmCarryCols];
   const u32 cl = threadIdx.x % kLmCarryCols, run = threadIdx.x / kLmCarryCols;
   const u32 colBlocks = (dim + kLmCarryCols - 1) / kLmCarryCols;
   for (u32 block = blockIdx.x; block < colBlocks; block += gridDim.x) {
@@ -561,35 +563,61 @@ __global__ void __launch_bounds__(kLmCarryCols * kLmCarryRuns) k_lm_scan_carry(c
         b[k] = aggB[at(ck)];
       }
     };
-    float W = 0.f, B = 0.f;
+    // the states behind the maps held in registers, from v on; s[k]: in front of map k.  (Two operations a map: v comes through
+    // whole or not at all, and the weight's part of it is taken off; what is not finite stays so, also behind a fresh map.)
+    auto states = [&](u32 cnt, float& v, float (&s)[kHold]) {
+      const float v0 = v;
+#pragma unroll
+      for (u32 k = 0; k < kHold; ++k) {
+        s[k] = v;
+        if (k < cnt) v = __builtin_fmaf(lm_map_whole(w[k]), v, __builtin_fmaf(lm_map_minus(w[k]), v, b[k]));
+      }
+      if (__builtin_expect(!lm_finite(v), 0)) {
+        v = v0;
+#pragma unroll
+        for (u32 k = 0; k < kHold; ++k) {
+          s[k] = v;
+          if (k < cnt) v = lm_map<true>(w[k], v, b[k]);
+        }
+      }
+    };
+    LmMap<1> m;
+    m.one();
+    float s[kHold];
     if (on) {
       for (u32 c = c0; c < c1; c += kHold) {
         load(c);
 #pragma unroll
         for (u32 k = 0; k < kHold; ++k) {
           if (c + k < c1) {
-            B = lm_map(w[k], B, b[k]);
-            W = lm_map_weight_then(W, w[k]);
+            m.pass(0, w[k]);
+            m.fresh = m.fresh || w[k] == kLmFresh;
           }
         }
+        states(c1 - c, m.B[0], s);
       }
     }
+    const float W = m.weight(0);
     s_W[run][cl] = W;
-    s_B[run][cl] = B;
+    s_k[run][cl] = lm_map_whole(W);
+    s_m[run][cl] = lm_map_minus(W);
+    s_B[run][cl] = m.B[0];
     __syncthreads();
     float v = 0.f;   // (no state enters the first chunk: its sentences begin inside it)
 #pragma unroll 8
-    for (u32 r = 0; r < run; ++r) v = lm_map(s_W[r][cl], v, s_B[r][cl]);
+    for (u32 r = 0; r < run; ++r) v = __builtin_fmaf(s_k[r][cl], v, __builtin_fmaf(s_m[r][cl], v, s_B[r][cl]));
+    if (__builtin_expect(!lm_finite(v), 0)) {
+      v = 0.f;
+#pragma unroll 1
+      for (u32 r = 0; r < run; ++r) v = lm_map<true>(s_W[r][cl], v, s_B[r][cl]);
+    }
     if (on) {
       for (u32 c = c0; c < c1; c += kHold) {
         if (per > kHold) load(c);
+        states(c1 - c, v, s);
 #pragma unroll
-        for (u32 k = 0; k < kHold; ++k) {
-          if (c + k < c1) {
-            aggB[at(c + k)] = v;
-            v = lm_map(w[k], v, b[k]);
-          }
-        }
+        for (u32 k = 0; k < kHold; ++k)
+          if (c + k < c1) aggB[at(c + k)] = s[k];
       }
     }
     __syncthreads();
@@ -625,11 +653,14 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_chunk(LmScan<T> q) {
     const u32 pack = cb * 64u + (u32)lane;
     const u32 col = lm_col<V>(pack < packs ? pack : packs - 1, q.dim);
     const u32 r0 = c * q.chunk, r1 = q.rows - r0 < q.chunk ? q.rows : r0 + q.chunk;
-    const u32 first = lm_offset(q.offsets, 0, q.rows);
-    u32 t = first > r0 ? first : r0;
-    if (t >= r1) continue;   // the batch begins behind the chunk
+    u32 t = r0, i = uni(lm_sentence_of(q.offsets, q.n, r0, lane));
+    if (i == q.n) {   // the batch begins behind r0
+      t = lm_offset(q.offsets, 0, q.rows);
+      if (t >= r1) continue;
+      i = uni(lm_sentence_of(q.offsets, q.n, t, lane));
+    }
     // From sentence to sentence; sentences without a row may be many, so they are passed over by a search.
-    for (u32 i = uni(lm_sentence_of(q.offsets, q.n, t, lane)); i < q.n;) {
+    while (i < q.n) {
       const u32 begin = lm_offset(q.offsets, i, q.rows), end = lm_offset(q.offsets, i + 1, q.rows), to = end < r1 ? end : r1;
       if (begin > t) t = begin;
       if (t >= to) break;   // (behind the last sentence)
@@ -660,10 +691,13 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_chunk(LmScan<T> q) 
     const u32 col = lm_col<V>(pack < packs ? pack : packs - 1, q.dim);
     const u32 r0 = c * q.chunk, r1 = q.rows - r0 < q.chunk ? q.rows : r0 + q.chunk;
     // sentences from the one with the last row down to the one with the first, those without a row passed over
-    const u32 total = lm_offset(q.offsets, q.n, q.rows);
-    u32 t = total < r1 ? total : r1;
-    if (t <= r0) continue;   // the batch ends in front of the chunk
-    for (u32 i = uni(lm_sentence_of(q.offsets, q.n, t - 1, lane)); i < q.n;) {
+    u32 t = r1, i = uni(lm_sentence_of(q.offsets, q.n, r1 - 1, lane));
+    if (i + 1 == q.n && lm_offset(q.offsets, q.n, q.rows) < r1) {   // the batch ends in front of r1
+      t = lm_offset(q.offsets, q.n, q.rows);
+      if (t <= r0) continue;
+      i = uni(lm_sentence_of(q.offsets, q.n, t - 1, lane));
+    }
+    while (i < q.n) {
       const u32 begin = lm_offset(q.offsets, i, q.rows), end = lm_offset(q.offsets, i + 1, q.rows);
       const u32 to = end < t ? end : t, from = begin > r0 ? begin : r0;
       if (from >= to) break;   // (in front of the first sentence)
