@@ -389,7 +389,7 @@ struct LmDiv {
 };
 
 constexpr u32 kLmThreads = 256;        // threads of a workgroup, where a kernel has no reason for another number
-constexpr u64 kLmChipBlocks = 256 * 8; // workgroups of kLmThreads threads that the 256 compute units hold at most
+constexpr u64 kLmChipBlocks = 256 * 8; // workgroups of kLmThreads threads that the 256 compute units hold, at up to 64 registers a lane
 constexpr u32 kLmMaxBlocks = 1u << 21; // largest grid (the sort of 2^31 entries has half of it); kernels that may need more loop
 
 }  // namespace jpp

@@ -85,7 +85,7 @@ struct Launcher {
 };
 
 // Results of more bytes than this leave with the non-temporal hint: 2 031 616 rows of 128 columns looked up in 101 us, without
-// it 162; the recurrence over 65 536 rows of 1 024 columns 129 us and 147, over 40 001 of 1 000 with its gradient 206 and 221.  Smaller
+// it 162; the recurrence over 65 536 rows of 1 024 columns 135 us and 152, over 40 001 of 1 000 with its gradient 220 and 236.  Smaller
 // ones stay where their reader finds them.
 constexpr u64 kStreamBytes = u64{64} << 20;
 bool streamed(u64 bytes) { return bytes > kStreamBytes; }
@@ -356,7 +356,7 @@ void launch_embed(Launcher& go, const jppgpu_lm_matrix* table, u32 vocab, u32 di
 
 // ---- the recurrence --------------------------------------------------------------------
 // Columns of a wavefront: a lane takes 4 of a long row, fewer where that leaves lanes idle (128 columns of floats with the
-// gradient: 464 us with two, 481 with one, 468 with four; 1 024 of bfloat16: 129 us with four, 159 with one).  The gradient
+// gradient: 464 us with two, 479 with one, 467 with four; 1 024 of bfloat16: 135 us with four, 163 with one).  The gradient
 // holds eight rows of five values an element in registers, so a lane takes 8 bytes a row there.
 u32 scan_pack(u32 dim, i32 type, bool grad) {
   const u32 most = grad && type == JPPGPU_LM_F32 ? 2 : 4;
@@ -366,9 +366,9 @@ u32 scan_pack(u32 dim, i32 type, bool grad) {
 
 // Whether the rows are walked in chunks, and of how many rows (0: a wavefront per sentence and column block).  Decided from
 // the sizes alone, not from the type, so that one workspace rule serves all.  Sentences of up to 256 rows are walked, and
-// longer ones where there are enough of about one length to fill the chip: a step of 64 sentences takes 10 us, 44 in chunks;
-// 16 384 sentences of 31 rows take 464 us either way, without the workspace.  Five documents of 40 001 rows of
-// 1 000 columns with the gradient: 206 us in chunks, 6.5 ms walked.  4 096 wavefronts: 6 144 and 8 192 took 6 % longer over 65 536
+// longer ones where there are enough of about one length to fill the chip: a step of 64 sentences takes 10 us, 46 in chunks;
+// 16 384 sentences of 31 rows of 128 floats with the gradient 464, 520 in chunks.  Five documents of 40 001 rows of
+// 1 000 columns with the gradient: 220 us in chunks, 8.1 ms walked.  4 096 wavefronts: 6 144 and 8 192 took 8 and 4 % longer over 65 536
 // rows of 1 024 columns.
 u32 scan_chunk(u64 rows, u64 n, u64 dim, u64 maxLen) {
   const u64 longest = maxLen == 0 || maxLen > rows ? rows : maxLen;
@@ -533,7 +533,8 @@ void launch_nce(Launcher& go, const LmNce& q, const void* h, const void* table, 
     go(k_lm_nce_score<T, V, G, NV, KIND>, div_up(q.n * div_up(q.cands, kLmScoreCands), kLmThreads / G), kLmThreads, q, hp, tp, ids);
     return;
   }
-  // no more workgroups than fit the chip at once: a wavefront that goes from token to token has the next one's data ahead
+  // at most kLmChipBlocks workgroups: a wavefront that goes from token to token has the next one's data ahead.  (These kernels
+  // have 82 to 181 registers a lane, so that a compute unit holds five to two of the eight workgroups at a time.)
   const u64 blocks = div_up(q.n, kLmThreads / 64), most = blocks < kLmChipBlocks ? blocks : kLmChipBlocks;
   if (dp != nullptr) go(k_lm_nce_loss<T, V, G, NV, KIND, true>, most, kLmThreads, q, hp, tp, ids, dp);
   else go(k_lm_nce_loss<T, V, G, NV, KIND, false>, most, kLmThreads, q, hp, tp, ids, dp);

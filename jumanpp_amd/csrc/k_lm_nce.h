@@ -10,8 +10,8 @@
 // four candidates side by side); longer rows take the whole wavefront (for 256 columns of 16 bits the loss would take three
 // times as long: a reduction over 64 lanes for every candidate, none side by side).
 // 507 904 tokens, 6 candidates, 128 bfloat16 columns are scored in 57 us: 0.72 GB asked of the L2s, 0.28 GB of it from outside,
-// the vector unit taking 0.6 of its slots.  The loss of 65 536 tokens, 33 candidates, 256 columns takes 107 us with dh, the
-// vector unit 0.74 of its slots: that is the bound there.  Hence the products in pairs (lm_dot2), addresses made once and
+// the vector unit taking 0.6 of its slots.  The loss of 65 536 tokens, 33 candidates, 256 columns takes 110 us with dh, the
+// vector unit 0.77 of its slots: that is the bound there.  Hence the products in pairs (lm_dot2), addresses made once and
 // handed on, and the exact row length as a kind of its own: 57 us against 70 with the masks of shorter rows; the loss gains
 // 35 us.
 #ifndef JPP_K_LM_NCE_H

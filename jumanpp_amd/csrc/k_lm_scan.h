@@ -15,10 +15,10 @@
 // afterwards, every eight rows, has them made again from the two weights, which is what the formula says of infinities.
 // The gradient runs backwards: with e the gradient of the state that reaches a row from behind,
 //     delta_t = dh_t + e, dx = delta b, dgate = delta (h_(t-1) - x) a b, e <- a delta.
-// Measured: 16 384 sentences of 31 rows of 128 floats, a wavefront each: 174 us with saved states, 291 us backwards, both
+// Measured: 16 384 sentences of 31 rows of 128 floats, a wavefront each: 175 us with saved states, 294 us backwards, both
 // 4.6 TB/s (a copy of sets beyond the caches reaches 4.8).  One sentence of 65 536 rows of 1 024 bfloat16 columns in chunks:
-// 55 us for the maps (4.9 TB/s), 6.5 for the states, 68 for the rows (5.9 TB/s).  Walked by one wavefront a column block it
-// takes 19.8 ms.
+// 59 us for the maps (4.6 TB/s, the vector unit at 0.7 of its slots), 8 for the states, 71 for the rows (5.7 TB/s).  Walked by
+// one wavefront a column block it takes 21.8 ms.
 // It needs h_(t-1) in 32 bits.  The forward pass leaves the state in front of every kLmSave-th row (an eighth of h's
 // elements); from there the gradient re-makes the states of kLmSave rows in registers, which costs fewer bytes than
 // reading h and does not see h's rounding to 16 bits.
@@ -538,8 +538,8 @@ __device__ __forceinline__ void lm_scan_enter(const LmScan<T>& q, u32 c, u32 col
 
 // The states between the groups: groupB[c] becomes the state that enters group c (BACK: from behind).  A workgroup owns 16
 // columns; 64 threads a column take consecutive runs of groups, first as one map each, then, from the state in front of
-// their run, state by state.  What a compute unit can have in flight bounds it, hence the groups: 10 us for the maps of
-// 1 024 chunks of 1 024 columns, 17 us with 64 columns a workgroup and 16 threads each.
+// their run, state by state.  What a compute unit can have in flight bounds it, hence the groups: 8 us for 256 groups of
+// 1 024 columns (for 1 024 chunks without groups 10, and 17 with 64 columns a workgroup and 16 threads each).
 constexpr u32 kLmCarryCols = 16, kLmCarryRuns = 64;
 template <bool BACK>
 __global__ void __launch_bounds__(kLmCarryCols * kLmCarryRuns) k_lm_scan_carry(const float* __restrict__ aggW, float* __restrict__ aggB, u32 chunks, u32 dim) {
