@@ -1258,6 +1258,31 @@ def scores_reach_the_lattice(E):
     assert sum(a != b for a, b in zip(mine, without)) >= 3, 'the scorer has to matter'
 
 
+@check(dtype=[F32, F16], dim=[130, 203, 262], max_len=[0, 1])
+def scan_not_finite_stays_in_its_column(E, dtype, dim, max_len):
+    """infinities and NaN next to every kind of column: of the same pack, of the pack that is moved back to the row's end, which two
+    lanes have; the other columns keep their bits"""
+    inf, nan = float('inf'), float('nan')
+    offsets, rows, gate, x, dh, state, dlast, _ = scan_inputs(([290, 0, 41], 3, 5), dim, dtype, dim)
+    od = E.to(offsets)
+
+    def run(gate, x, dh, state, dlast):
+        h, last, saved = lm.scan(E.to(gate), E.to(x), od, E.to(state), max_len=max_len, save=True, **E.kw)
+        return [t.cpu() for t in (h, last) + lm.scan_grad(E.to(gate), E.to(x), E.to(dh), saved, od, E.to(state), E.to(dlast), max_len=max_len, **E.kw)]
+
+    plain = run(gate, x, dh, state, dlast)
+    dirty = [1, 6, 127, 129, dim - 1, dim - 3, dim - 5]
+    x[20, 1], dh[100, 6], gate[200, 127], state[0, 129], dlast[0, dim - 1], x[300, dim - 3], gate[5, dim - 5] = inf, -inf, nan, inf, nan, -inf, nan
+    got = run(gate, x, dh, state, dlast)
+    again = run(gate, x, dh, state, dlast)
+    clean = torch.ones(dim, dtype=torch.bool)
+    clean[dirty] = False
+    for what, a, b, c in zip(('h', 'last', 'dgate', 'dx', 'dstate'), got, plain, again):
+        equal(what + ' of the other columns', a[:, clean], b[:, clean])
+        equal(what + ' again', a, c)
+        assert not a.isfinite().all(), what
+
+
 def run_all(device, lib_path, path=None):
     E = Env(device, lib_path)
     results = {}
