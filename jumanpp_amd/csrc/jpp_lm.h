@@ -260,7 +260,7 @@ __device__ __forceinline__ bool lm_finite(float v) { return __builtin_fabsf(v) <
 // gates in every chunk, and the same rounding of their product): 1 - A, or - A where that is the smaller.  kLmFresh: nothing of v
 // passes, also where v is no number.
 constexpr float kLmFresh = -2.f;
-__device__ __forceinline__ float lm_map_weight(float A, float C) { return C <= 0.5f ? C : -A; }   // C: 1 - A, made for itself
+__device__ __forceinline__ float lm_map_weight(float A, float C) { return A > 0.5f ? C : -A; }   // C: 1 - A, made for itself
 // A v + B = whole v + (minus v + B), for finite v
 __device__ __forceinline__ float lm_map_whole(float w) { return lm_open(w) ? 1.f : 0.f; }
 __device__ __forceinline__ float lm_map_minus(float w) { return w == kLmFresh ? 0.f : -w; }

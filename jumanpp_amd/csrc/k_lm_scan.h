@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kLmThreads) k_lm_scan_grad_seq(LmScan<T> q) {
 // ---- chunks ------------------------------------------------------------------------
 template <int V>
 struct LmMap {   // s -> A s + B
-  float A[V], C[V], B[V];   // C = 1 - A
+  float A[V], C[V], B[V];   // C = 1 - A as long as all weights are open ones; behind a closed one A is at most a half
   bool fresh;               // s -> B
   __device__ __forceinline__ void one() {
 #pragma unroll
@@ -338,7 +338,7 @@ struct LmMap {   // s -> A s + B
   }
   // the weight of this map, then of one of weight w
   __device__ __forceinline__ void pass(int e, float w) {
-    C[e] = __builtin_fmaf(w, A[e], lm_open(w) ? C[e] : 1.f);
+    C[e] = __builtin_fmaf(__builtin_fabsf(w), A[e], C[e]);
     A[e] = lm_kept(w, A[e]);
   }
   // this map, then the map (w, b)
