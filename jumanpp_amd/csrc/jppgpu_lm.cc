@@ -85,7 +85,7 @@ struct Launcher {
 };
 
 // Results of more bytes than this leave with the non-temporal hint: 2 031 616 rows of 128 columns looked up in 101 us, without
-// it 162; the recurrence over 65 536 rows of 1 024 columns 135 us and 152, over 40 001 of 1 000 with its gradient 220 and 236.  Smaller
+// it 162; the recurrence over 65 536 rows of 1 024 columns 134 us and 152, over 40 001 of 1 000 with its gradient 220 and 236.  Smaller
 // ones stay where their reader finds them.
 constexpr u64 kStreamBytes = u64{64} << 20;
 bool streamed(u64 bytes) { return bytes > kStreamBytes; }
@@ -356,7 +356,7 @@ void launch_embed(Launcher& go, const jppgpu_lm_matrix* table, u32 vocab, u32 di
 
 // ---- the recurrence --------------------------------------------------------------------
 // Columns of a wavefront: a lane takes 4 of a long row, fewer where that leaves lanes idle (128 columns of floats with the
-// gradient: 464 us with two, 479 with one, 467 with four; 1 024 of bfloat16: 135 us with four, 163 with one).  The gradient
+// gradient: 464 us with two, 479 with one, 467 with four; 1 024 of bfloat16: 134 us with four, 163 with one).  The gradient
 // holds eight rows of five values an element in registers, so a lane takes 8 bytes a row there.
 u32 scan_pack(u32 dim, i32 type, bool grad) {
   const u32 most = grad && type == JPPGPU_LM_F32 ? 2 : 4;
